@@ -19,6 +19,8 @@ LIB_PATH = os.environ.get("ESGPT_AMD_LIB", os.path.join(_HERE, "libesgpt_amd.so"
 ESGPT_OK, ESGPT_ERR_INVALID_ARG, ESGPT_ERR_LAUNCH, ESGPT_ERR_UNSUPPORTED = 0, 1, 2, 3
 F32, BF16 = 0, 1
 FLAG_BAD_INDEX, FLAG_TTE_NAN, FLAG_TTE_NO_OBS, FLAG_BAD_LABEL, FLAG_PEER_RANK = 1, 2, 4, 8, 16
+FLAG_BAD_PAGE = 32
+POS_F32, POS_I64 = 0, 1
 EMB_NORMALIZE, EMB_STATIC, EMB_TIME, EMB_CUMSUM, EMB_TIME_ABS = 1, 2, 4, 8, 16
 BAG_JOINT, BAG_CAT, BAG_NUM = 0, 1, 2
 TERM_SINGLE, TERM_MULTI, TERM_MVREG, TERM_UVREG = 1, 2, 3, 4
@@ -133,6 +135,12 @@ SIGNATURES = {
     "esgpt_kv_append": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp]),
     "esgpt_attn_decode": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                  _int, _vp]),
+    "esgpt_qk_norm_rope_fwd": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _i64, _f32, _vp, _int, _vp]),
+    "esgpt_qk_norm_rope_bwd_workspace": (_sz, [_i64, _i64, _i64, _i64, _int]),
+    "esgpt_qk_norm_rope_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp,
+                                      _sz, _int, _vp]),
+    "esgpt_kv_append_paged": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _i64, _f32, _vp, _vp, _vp, _i64, _vp, _vp, _i64,
+                                     _i64, _vp, _i64, _i64, _i64, _i64, _int, _vp, _vp]),
     "esgpt_residual_ln_partials": (_i64, [_i64]),
     "esgpt_residual_ln_fwd": (_int, [_vp, _vp, _int, _vp, _vp, _f32, _vp, _vp, _vp, _f32, _i64, _i64, _vp, _vp, _int,
                                      _vp, _vp, _vp]),

@@ -487,6 +487,157 @@ Tensor attn_decode(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_cac
   return o;
 }
 
+// ---- query / key norm + rotation, paged cache --------------------------------------------------------------------
+// Rows the kernels access 16 B at a time: contiguous, and copied once if a view's offset leaves them unaligned.
+Tensor rows16(const Tensor& t) {
+  Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+
+struct RopeIn {
+  Tensor q_w, k_w, pos, inv_freq;
+  int64_t R = 0;
+  int pos_dtype = ESGPT_POS_F32;
+};
+
+RopeIn rope_in(const char* what, const Tensor& x, int64_t rows0, int64_t rows1, int64_t hd,
+               const optional<Tensor>& q_w, const optional<Tensor>& k_w, const optional<Tensor>& pos,
+               const optional<Tensor>& inv_freq) {
+  auto has = [](const optional<Tensor>& t) { return t.has_value() && t->defined(); };
+  RopeIn r;
+  TORCH_CHECK(has(q_w) == has(k_w), what, ": q_w and k_w are given together or not at all");
+  if (has(q_w)) {
+    for (const Tensor* w : {&*q_w, &*k_w})
+      TORCH_CHECK(w->scalar_type() == at::kFloat && w->dim() == 1 && w->size(0) == hd && w->device() == x.device(), what,
+                  ": norm weights must be float32 of ", hd, " entries on the device of qkv");
+    r.q_w = q_w->contiguous();
+    r.k_w = k_w->contiguous();
+  }
+  TORCH_CHECK(has(pos) == has(inv_freq), what, ": pos and inv_freq are given together or not at all");
+  if (has(pos)) {
+    TORCH_CHECK(pos->scalar_type() == at::kFloat || pos->scalar_type() == at::kLong, what,
+                ": pos must be float32 (times) or int64 (indices)");
+    TORCH_CHECK(pos->dim() == 2 && pos->size(0) == rows0 && pos->size(1) == rows1 && pos->device() == x.device(), what,
+                ": pos must be [", rows0, ", ", rows1, "] on the device of qkv");
+    TORCH_CHECK(inv_freq->scalar_type() == at::kFloat && inv_freq->dim() == 1 && 2 * inv_freq->size(0) <= hd &&
+                    inv_freq->device() == x.device(),
+                what, ": inv_freq must be float32 with at most head size / 2 entries, on the device of qkv");
+    r.pos = pos->contiguous();
+    r.inv_freq = inv_freq->contiguous();
+    r.R = 2 * inv_freq->size(0);
+    r.pos_dtype = pos->scalar_type() == at::kLong ? ESGPT_POS_I64 : ESGPT_POS_F32;
+  }
+  return r;
+}
+
+const void* vptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const float* fptr(const Tensor& t) { return t.defined() ? ptr<const float>(t) : nullptr; }
+
+// Head size of a packed [B, T, 3D] buffer, checked.
+int64_t packed_hd(const char* what, const Tensor& qkv, int64_t H) {
+  require_hip(qkv, "qkv");
+  dtype_code(qkv.scalar_type());
+  TORCH_CHECK(qkv.dim() == 3 && H > 0 && qkv.size(2) % (3 * H) == 0 && qkv.size(2) > 0, what,
+              ": qkv must be [B, T, 3 * H * head size] with H = ", H);
+  return qkv.size(2) / 3 / H;
+}
+
+Tensor qk_norm_rope(const Tensor& qkv_, const optional<Tensor>& q_w, const optional<Tensor>& k_w,
+                    const optional<Tensor>& pos, const optional<Tensor>& inv_freq, int64_t H, double eps) {
+  const int64_t hd = packed_hd("esgpt.qk_norm_rope", qkv_, H);
+  const c10::DeviceGuard guard(qkv_.device());
+  const RopeIn r = rope_in("esgpt.qk_norm_rope", qkv_, qkv_.size(0), qkv_.size(1), hd, q_w, k_w, pos, inv_freq);
+  Tensor qkv = rows16(qkv_);
+  Tensor out = at::empty(qkv.sizes(), qkv.options());
+  check(esgpt_qk_norm_rope_fwd(qkv.data_ptr(), fptr(r.q_w), fptr(r.k_w), vptr(r.pos), r.pos_dtype, fptr(r.inv_freq), r.R,
+                               qkv.size(0) * qkv.size(1), H, hd, (float)eps, out.data_ptr(),
+                               dtype_code(qkv.scalar_type()), stream_of(qkv)),
+        "qk_norm_rope");
+  return out;
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rope_bwd(const Tensor& dout_, const Tensor& qkv_, const optional<Tensor>& q_w,
+                                            const optional<Tensor>& k_w, const optional<Tensor>& pos,
+                                            const optional<Tensor>& inv_freq, int64_t H, double eps) {
+  const int64_t hd = packed_hd("esgpt.qk_norm_rope_bwd", qkv_, H);
+  const c10::DeviceGuard guard(qkv_.device());
+  const RopeIn r = rope_in("esgpt.qk_norm_rope_bwd", qkv_, qkv_.size(0), qkv_.size(1), hd, q_w, k_w, pos, inv_freq);
+  TORCH_CHECK(dout_.sizes() == qkv_.sizes() && dout_.device() == qkv_.device(),
+              "esgpt.qk_norm_rope_bwd: dout must have the shape and device of qkv");
+  Tensor qkv = rows16(qkv_), dout = rows16(dout_.to(qkv_.scalar_type()));
+  const int64_t N = qkv.size(0) * qkv.size(1);
+  const int dt = dtype_code(qkv.scalar_type());
+  Tensor dqkv = at::empty(qkv.sizes(), qkv.options());
+  Tensor dw = at::empty({r.q_w.defined() ? 2 : 0, hd}, qkv.options().dtype(at::kFloat));
+  const size_t nb = r.q_w.defined() ? esgpt_qk_norm_rope_bwd_workspace(N, H, hd, r.R, dt) : 0;
+  Tensor ws = at::empty({(int64_t)nb}, qkv.options().dtype(at::kByte));
+  check(esgpt_qk_norm_rope_bwd(dout.data_ptr(), qkv.data_ptr(), fptr(r.q_w), fptr(r.k_w), vptr(r.pos), r.pos_dtype,
+                               fptr(r.inv_freq), r.R, N, H, hd, (float)eps, dqkv.data_ptr(), ptr<float>(dw),
+                               ws.data_ptr(), nb, dt, stream_of(qkv)),
+        "qk_norm_rope_bwd");
+  return {dqkv, dw};
+}
+
+// The two pools of a paged cache, [n_pages, H, page_size, hd]: updated in place, so never copied.
+void check_pages(const char* what, const Tensor& like, const Tensor& k_pages, const Tensor& v_pages) {
+  require_hip(like, what);
+  dtype_code(like.scalar_type());
+  TORCH_CHECK(k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes() && k_pages.size(1) > 0, what,
+              ": k_pages and v_pages must be [pages, heads, page size, head size] each");
+  for (const Tensor* t : {&k_pages, &v_pages})
+    TORCH_CHECK(t->scalar_type() == like.scalar_type() && t->device() == like.device() && t->is_contiguous() &&
+                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                what, ": the pages must be contiguous, 16-byte aligned, of the type and on the device of the rows");
+  const int64_t ps = k_pages.size(2);
+  TORCH_CHECK(ps >= 16 && ps <= 65536 && (ps & (ps - 1)) == 0, what, ": page size ", ps,
+              " is not a power of two from 16 to 65536");
+}
+
+void check_i32(const char* what, const char* name, const Tensor& t, const Tensor& like, int64_t dim, int64_t rows) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.size(0) == rows && t.is_contiguous() &&
+                  t.device() == like.device(),
+              what, ": ", name, " must be a contiguous int32 tensor with ", rows, " rows on the device of the rows");
+}
+
+Tensor row_mask_of(const char* what, const optional<Tensor>& m, const Tensor& like, int64_t S, int64_t Lq) {
+  if (!m.has_value() || !m->defined()) return Tensor();
+  TORCH_CHECK(m->scalar_type() == at::kBool && m->dim() == 2 && m->size(0) == S && m->size(1) == Lq &&
+                  m->device() == like.device(),
+              what, ": row_mask must be bool [", S, ", ", Lq, "] on the device of the rows");
+  return m->contiguous();
+}
+
+int32_t* err_of(const char* what, const Tensor& err, const Tensor& like) {
+  TORCH_CHECK(err.device() == like.device() && err.is_contiguous() && err.nbytes() >= 16, what,
+              ": err must be the device's error block (eventstreamgpt_amd.kernels.err_word)");
+  return reinterpret_cast<int32_t*>(err.data_ptr());
+}
+
+Tensor kv_append_paged(const Tensor& qkv_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                       const Tensor& past, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
+                       const optional<Tensor>& k_w, const optional<Tensor>& pos, const optional<Tensor>& inv_freq,
+                       double eps, const Tensor& err) {
+  const char* what = "esgpt.kv_append_paged";
+  check_pages(what, qkv_, k_pages, v_pages);
+  const int64_t H = k_pages.size(1), hd = packed_hd(what, qkv_, H), S = qkv_.size(0), Lq = qkv_.size(1);
+  TORCH_CHECK(hd == k_pages.size(3), what, ": the pages hold heads of ", k_pages.size(3), ", qkv of ", hd);
+  const c10::DeviceGuard guard(qkv_.device());
+  const RopeIn r = rope_in(what, qkv_, S, Lq, hd, q_w, k_w, pos, inv_freq);
+  check_i32(what, "page_table", page_table, qkv_, 2, S);
+  check_i32(what, "past", past, qkv_, 1, S);
+  Tensor m = row_mask_of(what, row_mask, qkv_, S, Lq);
+  int32_t* e = err_of(what, err, qkv_);
+  Tensor qkv = rows16(qkv_);
+  Tensor q = at::empty({S, Lq, H * hd}, qkv.options());
+  check(esgpt_kv_append_paged(qkv.data_ptr(), fptr(r.q_w), fptr(r.k_w), vptr(r.pos), r.pos_dtype, fptr(r.inv_freq), r.R,
+                              (float)eps, m.defined() ? ptr<const uint8_t>(m) : nullptr, ptr<const int32_t>(past),
+                              ptr<const int32_t>(page_table), page_table.size(1), k_pages.data_ptr(),
+                              v_pages.data_ptr(), k_pages.size(0), k_pages.size(2), q.data_ptr(), S, Lq, H, hd,
+                              dtype_code(qkv.scalar_type()), e, stream_of(qkv)),
+        "kv_append_paged");
+  return q;
+}
+
 // ---- output-layer losses -------------------------------------------------------------------------------------------
 std::vector<esgpt_loss_term> make_terms(at::IntArrayRef t) {
   TORCH_CHECK(t.size() % 8 == 0, "terms: 8 ints per term");
@@ -1076,6 +1227,11 @@ TORCH_LIBRARY(esgpt, m) {
   m.def("kv_append(Tensor qkv, Tensor(a!) k_cache, Tensor(b!) v_cache, int past) -> ()");
   m.def("attn_decode(Tensor qkv, Tensor k_cache, Tensor v_cache, Tensor? key_mask, Tensor? query_mask, int H, "
         "int Lk, int window) -> Tensor");
+  m.def("qk_norm_rope(Tensor qkv, Tensor? q_w, Tensor? k_w, Tensor? pos, Tensor? inv_freq, int H, float eps) -> Tensor");
+  m.def("qk_norm_rope_bwd(Tensor dout, Tensor qkv, Tensor? q_w, Tensor? k_w, Tensor? pos, Tensor? inv_freq, int H, "
+        "float eps) -> (Tensor, Tensor)");
+  m.def("kv_append_paged(Tensor qkv, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor past, "
+        "Tensor? row_mask, Tensor? q_w, Tensor? k_w, Tensor? pos, Tensor? inv_freq, float eps, Tensor err) -> Tensor");
   m.def("output_loss(Tensor zc, Tensor? zt, Tensor? zc_bias, " BATCH_SCHEMA ", int n_levels, int shift, int[] terms, "
         "int[] tte_i, float[] tte_f, Tensor err, int path=0) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("residual_ln(Tensor? x, Tensor? y, Tensor? bias, Tensor ln_w, Tensor ln_b, Tensor? row_mask, float p, "
@@ -1137,6 +1293,9 @@ TORCH_LIBRARY_IMPL(esgpt, CUDA, m) {
   m.impl("attention_bwd", &attention_bwd);
   m.impl("kv_append", &kv_append);
   m.impl("attn_decode", &attn_decode);
+  m.impl("qk_norm_rope", &qk_norm_rope);
+  m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
+  m.impl("kv_append_paged", &kv_append_paged);
   m.impl("output_loss", &output_loss);
   m.impl("residual_ln", &residual_ln);
   m.impl("residual_ln_bwd", &residual_ln_bwd);

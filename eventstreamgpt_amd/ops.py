@@ -15,6 +15,8 @@ Differentiable operators and the reference code they replace:
 ``embed_epilogue``    temporal encoding / level cumsum / mask after the SPLIT projection (the bf16 / f32 SPLIT
                       path runs ``split_proj_prep`` + GEMM + ``embed_epilogue`` in kernels._SplitProjection)
 ``attention``         InnerSelfAttention._attn (transformer.py:171-217) on a packed q|k|v buffer
+``qk_norm_rope``      RMS norm of the queries and keys per head and their rotation by the events' positions, on the
+                      packed q|k|v buffer that ``attention`` reads (not in the reference: opt-in)
 ``residual_ln``       residual + resid dropout + event mask + LayerNorm (transformer.py:350-461, 810-831)
 ``bias_act``          c_fc bias + activation (transformer.py:378-391)
 ``linear``            a bias-optional projection on the bf16 weight shadow, gradients to the f32 parameters
@@ -29,9 +31,9 @@ Used by the NA glue's autograd Functions (transformer/structured_attention.py): 
 ``na_assemble`` / ``na_assemble_bwd`` (structured_attention.py:63-156).
 
 Non-differentiable: ``embed_bag_bwd``, ``embed_epilogue_bwd``, ``attention_bwd``, ``residual_ln_bwd``,
-``bias_act_bwd``, ``linear_act``, ``linear_bwd`` (+ ``weight_grad_join``: with ``dw_tickets`` the weight gradient
+``bias_act_bwd``, ``qk_norm_rope_bwd``, ``linear_act``, ``linear_bwd`` (+ ``weight_grad_join``: with ``dw_tickets`` the weight gradient
 runs on a second stream, joined by that op), ``gemm`` / ``gemm_``, ``column_sum``, ``kv_append``,
-``attn_decode`` (generation), ``pack`` (the compute-dtype parameter copies) and ``adamw``
+``attn_decode`` (generation), ``kv_append_paged`` (the same norm and rotation into a paged cache), ``pack`` (the compute-dtype parameter copies) and ``adamw``
 (generative_modeling.py:460-485).
 
 There is no CPU kernel: calling an operator on CPU tensors raises (no fallback).
@@ -50,7 +52,7 @@ ACT_DERIV = 8  # ESGPT_ACT_DERIV (include/esgpt_amd.h): the pre-activation buffe
 _state = {"loaded": False}
 
 OPS = ("embed_joint", "embed_split_bags", "embed_epilogue", "embed_epilogue_bwd", "embed_bag_bwd", "attention",
-       "attention_bwd", "kv_append", "attn_decode", "output_loss", "residual_ln", "residual_ln_bwd", "bias_act",
+       "attention_bwd", "kv_append", "attn_decode", "qk_norm_rope", "qk_norm_rope_bwd", "kv_append_paged", "output_loss", "residual_ln", "residual_ln_bwd", "bias_act",
        "bias_act_bwd", "column_sum", "gemm", "gemm_", "linear_act", "linear_bwd", "linear", "mlp", "head_loss",
        "pack", "adamw", "adamw_dev", "weight_grad_join", "residual_ln_bwd_partials", "colsum_flush", "seed_bank", "residual",
        "residual_bwd", "na_split", "na_split_bwd_", "na_assemble", "na_assemble_bwd", "na_head_split",
@@ -237,6 +239,19 @@ def _register():
 
     @fake(lib + "attn_decode")
     def _(qkv, k_cache, v_cache, key_mask, query_mask, H, Lk, window):
+        return qkv.new_empty(qkv.shape[0], qkv.shape[1], qkv.shape[2] // 3)
+
+    @fake(lib + "qk_norm_rope")
+    def _(qkv, q_w, k_w, pos, inv_freq, H, eps):
+        return torch.empty_like(qkv, memory_format=torch.contiguous_format)
+
+    @fake(lib + "qk_norm_rope_bwd")
+    def _(dout, qkv, q_w, k_w, pos, inv_freq, H, eps):
+        return (torch.empty_like(qkv, memory_format=torch.contiguous_format),
+                qkv.new_empty(0 if q_w is None else 2, qkv.shape[2] // 3 // H, dtype=torch.float32))
+
+    @fake(lib + "kv_append_paged")
+    def _(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err):
         return qkv.new_empty(qkv.shape[0], qkv.shape[1], qkv.shape[2] // 3)
 
     def _loss_fake(zc, zt, shift, n_terms, B):
@@ -447,6 +462,23 @@ def _register():
         return dqkv, None, None, None, None, None, None, None
 
     reg(lib + "attention", _at_bwd, setup_context=_at_setup)
+
+    # qk_norm_rope: d qkv from the raw buffer (the norms are recomputed), d q_w and d k_w summed in a fixed order
+    def _qr_setup(ctx, inputs, output):
+        qkv, q_w, k_w, pos, inv_freq, H, eps = inputs
+        if ctx.needs_input_grad[3] or ctx.needs_input_grad[4]:
+            raise NotImplementedError("eventstreamgpt_amd: qk_norm_rope has no gradient for pos and inv_freq")
+        ctx.save_for_backward(qkv, q_w, k_w, pos, inv_freq)
+        ctx.meta = (H, eps)
+
+    def _qr_bwd(ctx, dout):
+        H, eps = ctx.meta
+        qkv, q_w, k_w, pos, inv_freq = ctx.saved_tensors
+        dqkv, dw = ops.qk_norm_rope_bwd(dout, qkv, q_w, k_w, pos, inv_freq, H, eps)
+        dq_w, dk_w = (None, None) if q_w is None else (dw[0], dw[1])
+        return dqkv, dq_w, dk_w, None, None, None, None
+
+    reg(lib + "qk_norm_rope", _qr_bwd, setup_context=_qr_setup)
 
     # residual: d x (all rows of x; zeros for the rows skip_T leaves out), d y (y's dtype)
     def _rs_setup(ctx, inputs, output):

@@ -44,6 +44,12 @@ extern "C" {
 #define ESGPT_FLAG_BAD_LABEL 8    /* classification / regression target outside its vocabulary slice      */
 #define ESGPT_FLAG_PEER_RANK 16   /* set by the host DDP exchange: another rank's step raised a flag         */
 
+#define ESGPT_FLAG_BAD_PAGE 32    /* paged cache: a page id outside the pool, or a length outside its page table  */
+
+/* position types of the rotation */
+#define ESGPT_POS_F32 0           /* event times                                                           */
+#define ESGPT_POS_I64 1           /* indices (|pos| < 2^29 keeps the angle's product exact)                */
+
 /* embedding flags */
 #define ESGPT_EMB_NORMALIZE 1     /* do_normalize_by_measurement_index                                     */
 #define ESGPT_EMB_STATIC 2        /* StaticEmbeddingMode.SUM_ALL                                           */
@@ -221,6 +227,37 @@ int esgpt_kv_append(const void* qkv, int64_t ld_qkv, void* k_cache, void* v_cach
 int esgpt_attn_decode(const void* q, int64_t ld_q, const void* k_cache, const void* v_cache, const uint8_t* key_mask,
                       const uint8_t* query_mask, void* o, int64_t ld_o, int64_t B, int64_t H, int64_t Lq, int64_t Lk,
                       int64_t cap, int64_t hd, int64_t window, int dtype, void* stream);
+
+/* ---- Query / key norm and rotation, paged cache --------------------------------------------------------------
+ * esgpt_qk_norm_rope_fwd: the packed q|k|v rows qkv [N, 3D] (D = H*hd) -> out [N, 3D] with every head of q and of k
+ *   z = w * x / sqrt(mean(x^2) + eps)   (q_w, k_w: f32 [hd], both or neither; neither: z = x), then rotated by the
+ *   token's position over its first R dimensions: (z_i, z_{i+R/2}) by the angle pos * inv_freq_i, i < R/2 (angles in
+ *   f64: the product is exact, event times reach 1e6 minutes); v is copied. out is what esgpt_attn_fwd reads, whose
+ *   scores are not scaled by 1/sqrt(hd). pos: [N], pos_dtype ESGPT_POS_F32 / _I64; inv_freq: f32 [R/2]; R = 0: no
+ *   rotation (pos, inv_freq may be NULL). hd <= 128, hd % 8 == 0 (bf16) or hd % 4 == 0 (f32), H*hd <= 16384, R even
+ *   and <= hd; 16-B aligned buffers; out apart from qkv.
+ * esgpt_qk_norm_rope_bwd: from the raw rows and dout [N, 3D]: dqkv [N, 3D] and, with weights,
+ *   dw f32 [2, hd] = (d q_w, d k_w), summed in a fixed order (workspace: esgpt_qk_norm_rope_bwd_workspace bytes).
+ * esgpt_kv_append_paged: the same norm and rotation of S sequences' new rows qkv [S, Lq, 3D] on the way into a paged
+ *   cache. k_pages / v_pages: [n_pages, H, page_size, hd] (a head's rows of one page are contiguous; page_size a
+ *   power of two, 16..65536); page_table int32 [S, table_w]. Row i of sequence s goes to cache row past[s] + (rows
+ *   before i that row_mask [S, Lq] keeps; NULL: all), i.e. padded rows are not stored; q [S, Lq, D] gets the
+ *   normalised, rotated queries (zeros in padded rows). A row beyond the table, a negative past or a page outside
+ *   [0, n_pages) raises ESGPT_FLAG_BAD_PAGE and is not stored. Cache rows must be distinct: two sequences that name
+ *   the same page and write the same row of it leave either's values there. */
+int esgpt_qk_norm_rope_fwd(const void* qkv, const float* q_w, const float* k_w, const void* pos, int pos_dtype,
+                           const float* inv_freq, int64_t R, int64_t N, int64_t H, int64_t hd, float eps, void* out,
+                           int dtype, void* stream);
+size_t esgpt_qk_norm_rope_bwd_workspace(int64_t N, int64_t H, int64_t hd, int64_t R, int dtype);
+int esgpt_qk_norm_rope_bwd(const void* dout, const void* qkv, const float* q_w, const float* k_w, const void* pos,
+                           int pos_dtype, const float* inv_freq, int64_t R, int64_t N, int64_t H, int64_t hd,
+                           float eps, void* dqkv, float* dw, void* workspace, size_t workspace_bytes, int dtype,
+                           void* stream);
+int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, const void* pos, int pos_dtype,
+                          const float* inv_freq, int64_t R, float eps, const uint8_t* row_mask, const int32_t* past,
+                          const int32_t* page_table, int64_t table_w, void* k_pages, void* v_pages, int64_t n_pages,
+                          int64_t page_size, void* q, int64_t S, int64_t Lq, int64_t H, int64_t hd, int dtype,
+                          int32_t* err, void* stream);
 
 /* ---- Output layer losses -----------------------------------------------------------------------------------
  * GenerativeOutputLayerBase.get_{classification,regression,TTE}_outputs (model_output.py:1311-1721) with
