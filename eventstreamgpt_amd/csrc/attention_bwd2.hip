@@ -263,8 +263,10 @@ struct DqCfg {
   static constexpr int MERGE = 2 * (HDP / 32) * 16 * 64 * 2;  // bf16 elements holding the f32 merge state
 };
 
+// hd 64 with keep bits (tools build only: split2_keys keeps dropout at hd 64 on the fused kernel) needs more than the 256
+// registers of two workgroups per CU without packed-f32 instructions.
 template <int HD, int DM>
-__global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void attn_bwd_dq_kernel(
+__global__ __launch_bounds__(256, HD == 128 || (HD == 64 && DM == DROP_BITS) ? 1 : 2) void attn_bwd_dq_kernel(
     const __bf16* __restrict__ q, const __bf16* __restrict__ k, const __bf16* __restrict__ v, int64_t ld_in,
     int64_t tq, const __bf16* __restrict__ o, int64_t ld_o, const __bf16* __restrict__ dout, int64_t ld_do,
     const float* __restrict__ lse, const uint8_t* __restrict__ kmask, const uint8_t* __restrict__ qmask,
