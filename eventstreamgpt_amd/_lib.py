@@ -141,6 +141,9 @@ SIGNATURES = {
                                       _sz, _int, _vp]),
     "esgpt_kv_append_paged": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _i64, _f32, _vp, _vp, _vp, _i64, _vp, _vp, _i64,
                                      _i64, _vp, _i64, _i64, _i64, _i64, _int, _vp, _vp]),
+    "esgpt_attn_decode_shared_workspace": (_sz, [_i64] * 8 + [_int]),
+    "esgpt_attn_decode_shared": (_int, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64,
+                                        _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp, _sz, _vp, _vp]),
     "esgpt_residual_ln_partials": (_i64, [_i64]),
     "esgpt_residual_ln_fwd": (_int, [_vp, _vp, _int, _vp, _vp, _f32, _vp, _vp, _vp, _f32, _i64, _i64, _vp, _vp, _int,
                                      _vp, _vp, _vp]),

@@ -1,0 +1,754 @@
+// Attention of newly generated events over a paged cache in which n trajectories share one subject's history.
+//
+// generate(num_return_sequences = n) continues every subject n times from the same history. Group g's history is kept
+// once (prefix pages, P_g rows); trajectory s = g n .. g n + n - 1 has its own pages (own rows). A new event i of s at
+// own row t_i sees every history row and own rows <= t_i, inside the window if there is one (index distance < window):
+//   o = sum_j e^{q.k_j - m} v_j / sum_j e^{q.k_j - m},  m = max_j q.k_j   (no 1/sqrt(hd), as esgpt_attn_fwd)
+//
+// The bound is HBM: 2 hd s bytes per history row and head ONCE per group, and the same per own row. So the rows of a
+// group (n trajectories x Lq events) are the columns of one matrix product: S^T = K Q^T and O^T = V^T P^T on the 16-wide
+// MFMAs, where lane l holds column (query row) l % 16 and keys 4 (l / 16) .. + 3 of a 16-key tile, so a row's softmax
+// statistics are lane-local but for two lane swaps, and P goes from the accumulator to the next product's operand
+// without leaving its lane. An own row is one column of sixteen: 15/16 of the MFMA rate idles there, which costs
+// nothing as long as memory is the bound (a bf16 tile of 16 keys x 64 takes 64 MFMA cycles for 4 KB, 64 B per cycle and
+// SIMD, against the 13 B per cycle that HBM gives a whole CU).
+//
+// Split: the history of each (group, head, 16 or 32 rows) is cut into chunks (one workgroup each, its four waves taking
+// every fourth 32-key block and joining through LDS), the own rows of each (trajectory, head) into chunks of one wave.
+// Each part leaves (m, l, O) in f32 and a second kernel joins a row's parts; with one part in all the result is
+// written directly. The cut follows the caller's bounds on the lengths (the lengths themselves are on the device).
+//
+// Nothing is read beyond a sequence's length: rows past it are zeros in registers, so what an unused part of a page
+// holds (NaN, infinity) never meets a product. Where a tile is partly masked (a window's edge, a later event of the same
+// call), 0 x infinity is kept out of the other rows by an exact path (masked_pv).
+#include "common.h"
+
+#include <algorithm>
+
+using namespace esgpt;
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kMaxLq = 16;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct SharedArgs {
+  const void *q, *kp, *vp;
+  void* o;
+  const int32_t *prefix_table, *prefix_lens, *table, *past;
+  const uint8_t* row_mask;  // [S, Lq] or null
+  float* ml;                // [S Lq H, NP, 2] (m, l)
+  float* po;                // [S Lq H, NP, hd]
+  int32_t* err;
+  int64_t n_pages, prefix_w, table_w;
+  int S, n, Lq, H, hd, psl;     // psl: log2 of the page size
+  int prefix_cap, cap, window;  // window 0: none
+  int M, RT;                    // rows of a group; row tiles of the history's workgroups
+  int NPc, NSc, NP, pchunk, schunk;
+  int units;  // history workgroups; the own rows' follow
+};
+
+__device__ __forceinline__ float xmax(float v) {  // over the four lanes of one column
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float xsum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) { return -wave_min_i(-v); }
+
+// One new event: its place among its trajectory's own rows. active: it exists, is not padding and its past is sane.
+struct Row {
+  int64_t out;  // row of q and o
+  int at;       // own row
+  bool active;
+};
+__device__ __forceinline__ Row row_of(const SharedArgs& a, int s, int i, bool exists) {
+  Row r{0, 0, false};
+  if (!exists) return r;
+  r.out = (int64_t)s * a.Lq + i;
+  const int past = a.past[s];
+  int k = i;
+  bool keep = true;
+  if (a.row_mask) {
+    k = 0;
+    for (int j = 0; j < i; ++j) k += a.row_mask[(int64_t)s * a.Lq + j] != 0;
+    keep = a.row_mask[r.out] != 0;
+  }
+  if (!keep) return r;
+  if (past < 0 || past > a.cap - 1 - k) {  // a row that the cache has no place for
+    set_err(a.err, ESGPT_FLAG_BAD_PAGE);
+    if (past < 0) return r;
+  }
+  r.at = min(past, a.cap) + k;
+  r.active = true;
+  return r;
+}
+__device__ __forceinline__ int prefix_len(const SharedArgs& a, int g) {
+  if (a.prefix_cap == 0) return 0;
+  const int P = a.prefix_lens[g];
+  if (P < 0 || P > a.prefix_cap) set_err(a.err, ESGPT_FLAG_BAD_PAGE);
+  return min(max(P, 0), a.prefix_cap);
+}
+
+// Dimension of accumulator register r of tile dt in lane group g (= lane / 16). bf16: the transposed V tile's natural
+// rows. f32: tiles 2p and 2p + 1 hold the even and odd dimensions of 32p .. 32p + 31, so that a lane reads V in pairs.
+template <typename T>
+__device__ __forceinline__ int dim_of(int dt, int g, int r) {
+  if constexpr (sizeof(T) == 2) return 16 * dt + 4 * g + r;
+  else return 32 * (dt >> 1) + 2 * (4 * g + r) + (dt & 1);
+}
+
+// Four neighbouring dimensions dim .. dim + 3 of one column: of tile d in bf16; in f32, registers 2 (d & 1) and
+// 2 (d & 1) + 1 of the pair of tiles that d belongs to.
+template <typename T, int DT>
+__device__ __forceinline__ float4 four(const f32x4 (&acc)[DT], int d, int g, int& dim) {
+  if constexpr (sizeof(T) == 2) {
+    dim = 16 * d + 4 * g;
+    return make_float4(acc[d][0], acc[d][1], acc[d][2], acc[d][3]);
+  } else {
+    const int p = d & ~1, r = 2 * (d & 1);
+    dim = 16 * p + 8 * g + 2 * r;
+    return make_float4(acc[p][r], acc[p + 1][r], acc[p][r + 1], acc[p + 1][r + 1]);
+  }
+}
+
+template <typename T, int KD, int NT>
+struct Walk {
+  static constexpr bool kBf16 = sizeof(T) == 2;
+  static constexpr int KT = kBf16 ? 2 : 1;  // 16-key tiles per block: both types move 8 KB (hd 64) per block and wave
+  static constexpr int KB = 16 * KT;
+  static constexpr int DT = 2 * KD;      // 16-wide tiles of the head
+  static constexpr int LD = KD * 32 + 16;  // LDS row of V (elements): 8 mod 16 dwords, transposed reads hit all banks
+
+  const SharedArgs& a;
+  int h, lane, g, c;  // g = lane / 16, c = lane % 16
+  __bf16* vt;         // bf16: this wave's V tile, KB x LD
+  f32x4 acc[NT][DT];
+  float m[NT], l[NT];
+  uint4 qf[NT][kBf16 ? KD : 2 * KD];
+
+  __device__ __forceinline__ Walk(const SharedArgs& a_, int h_, void* lds) : a(a_), h(h_) {
+    lane = lane_id();
+    g = lane >> 4;
+    c = lane & 15;
+    vt = reinterpret_cast<__bf16*>(lds);
+    offsets();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // Queries: column c of tile t is row `out` of q. bf16: chunk kd holds dims 32 kd + 8 g .. + 7; f32: chunk k holds
+  // dims 16 k + 4 g .. + 3 (the products contract over lane groups, in this permuted order on both sides).
+  __device__ __forceinline__ void load_q(int t, const Row& r) {
+    constexpr int NQ = kBf16 ? KD : 2 * KD, E = kBf16 ? 8 : 4;
+    const T* p = reinterpret_cast<const T*>(a.q) + (r.out * a.H + h) * a.hd;
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) {
+      const int d = k * 4 * E + E * g;
+      qf[t][k] = (r.active && d < a.hd) ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  static constexpr int NK = kBf16 ? KD : 2 * KD;        // 16-B chunks of a key that a lane holds
+  static constexpr int LPR = KD == 3 ? 16 : 4 * KD;      // bf16: lanes that read one row of V (12 of 16 at 96)
+  static constexpr int NV = kBf16 ? LPR / 2 : 2 * KD;    // bf16: 16-B loads of a block's V; f32: 16-B register groups
+
+  struct Block {
+    uint4 k[KT * NK], v[NV];
+    const T* vb[KT];  // first row of each tile's values
+    bool ok[KT];      // false: a bad page
+  };
+
+  // Byte offsets of this lane's chunks in a 16-row tile; beyond the head's width: out of every range (reads zero).
+  static constexpr int kOut = 1 << 30;
+  int ko[NK], vo[kBf16 ? 1 : KD];
+  __device__ __forceinline__ void offsets() {
+    constexpr int E = kBf16 ? 8 : 4;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const int d = k * 4 * E + E * g;
+      ko[k] = d < a.hd ? (c * a.hd + d) * (int)sizeof(T) : kOut;
+    }
+    if constexpr (kBf16) {
+      const int d = (lane % LPR) * 8;
+      vo[0] = d < a.hd ? (lane / LPR * a.hd + d) * 2 : kOut;
+    } else {
+#pragma unroll
+      for (int p = 0; p < KD; ++p) {
+        const int d = 32 * p + 2 * c;
+        vo[p] = d < a.hd ? (4 * g * a.hd + d) * 4 : kOut;
+      }
+    }
+  }
+
+  // Loads the block at key k0 by range-checked buffer loads: zeros past k_end and on a bad page. pid: page ids of this
+  // round of blocks, lane slot * KT + tile.
+  __device__ __forceinline__ void load(Block& b, int k0, int k_end, int pid, int slot) {
+    const int rb = a.hd * (int)sizeof(T);
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const int id = __builtin_amdgcn_readlane(pid, slot * KT + t);
+      b.ok[t] = id >= 0;
+      const int64_t row = b.ok[t] ? (((int64_t)id * a.H + h) << a.psl) + ((k0 + 16 * t) & ((1 << a.psl) - 1)) : 0;
+      const int n = b.ok[t] ? min(16, max(0, k_end - k0 - 16 * t)) * rb : 0;
+      const T* kb = reinterpret_cast<const T*>(a.kp) + row * a.hd;
+      b.vb[t] = reinterpret_cast<const T*>(a.vp) + row * a.hd;
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kb), (short)0, n, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rv =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(b.vb[t]), (short)0, n, 0x00020000);
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+        b.k[t * NK + k] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko[k], 0, 0));
+      if constexpr (kBf16) {
+#pragma unroll
+        for (int i = 0; i < NV / 2; ++i)
+          b.v[t * (NV / 2) + i] = __builtin_bit_cast(
+              uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, vo[0] + i * (64 / LPR) * rb, 0, 0));
+      } else {
+        float2* v = reinterpret_cast<float2*>(b.v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int p = 0; p < KD; ++p)
+            v[e * KD + p] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rv, vo[p] + e * rb, 0, 0));
+      }
+    }
+  }
+
+  __device__ __forceinline__ static bool nonfinite(const Block& b) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t w[4] = {b.v[i].x, b.v[i].y, b.v[i].z, b.v[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bad |= (w[j] & 0x7f800000u) == 0x7f800000u;
+        if (kBf16) bad |= (w[j] & 0x7f80u) == 0x7f80u;
+      }
+    }
+    return bad;
+  }
+
+  // P.V of a partly masked block whose values are not all finite, key by key: a key adds nothing (not even
+  // 0 x infinity) to the rows that do not see it. Rare: reads the values again.
+  __device__ __forceinline__ void masked_pv(const Block& b, const float (&p)[4 * KT], f32x4 (&o)[DT], int k0, int lo,
+                                            int hi) {
+#pragma nounroll
+    for (int i = 0; i < 4 * KT; ++i) {
+      float pi = p[0];
+#pragma unroll
+      for (int j = 1; j < 4 * KT; ++j) pi = i == j ? p[j] : pi;
+      if (!(i < 4 ? b.ok[0] : b.ok[KT - 1])) continue;
+      const T* vb = i < 4 ? b.vb[0] : b.vb[KT - 1];
+#pragma nounroll
+      for (int gg = 0; gg < 4; ++gg) {
+        const float pk = to_f32(from_f32<T>(__shfl(pi, 16 * gg + c, 64)));
+        const int row = 4 * gg + (i & 3), key = k0 + (i & ~3) * 4 + row;
+        if (key < lo || key >= hi) continue;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int dim = dim_of<T>(d, g, x);
+            if (dim < a.hd) o[d][x] = fmaf(pk, to_f32(vb[row * a.hd + dim]), o[d][x]);
+          }
+      }
+    }
+  }
+
+  // Scores, online softmax and P.V of one block. Row (column c of tile t) sees keys [lo[t], hi[t]). full: every row
+  // sees the whole block.
+  __device__ __forceinline__ void step(const Block& b, int k0, const int (&lo)[NT], const int (&hi)[NT], bool full) {
+    bool slow = false;
+    if (!full) slow = __any(nonfinite(b));
+    if constexpr (kBf16) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int row = i * (64 / LPR) + lane / LPR, d = (lane % LPR) * 8;
+        if (KD != 3 || d < 32 * KD) *reinterpret_cast<uint4*>(vt + row * LD + d) = b.v[i];
+      }
+    }
+    float p[NT][4 * KT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      f32x4 s[KT];
+#pragma unroll
+      for (int u = 0; u < KT; ++u) {
+        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (kBf16) {
+#pragma unroll
+          for (int k = 0; k < KD; ++k)
+            s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.k[u * KD + k]),
+                                                           __builtin_bit_cast(bf16x8, qf[t][k]), s[u], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2 * KD; ++k) {
+            const f32x4 kf = __builtin_bit_cast(f32x4, b.k[k]), q4 = __builtin_bit_cast(f32x4, qf[t][k]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], q4[e], s[u], 0, 0, 0);
+          }
+        }
+      }
+      uint32_t vis = 0xffffffffu;
+      float mx = -INFINITY;
+      if (!full) {
+        vis = 0;
+#pragma unroll
+        for (int u = 0; u < KT; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = k0 + 16 * u + 4 * g + r;
+            if (key >= lo[t] && key < hi[t] && b.ok[u]) vis |= 1u << (4 * u + r);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4 * KT; ++i) {
+        const float x = s[i >> 2][i & 3];
+        mx = fmaxf(mx, (full || (vis >> i & 1)) ? x : -INFINITY);
+      }
+      const float mn = fmaxf(m[t], xmax(mx));
+      const float mc = mn == -INFINITY ? 0.f : mn * kLog2e;
+      if (__any(mn != m[t])) {
+        const float f = __builtin_amdgcn_exp2f(fmaf(m[t], kLog2e, -mc));
+        l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+        m[t] = mn;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4 * KT; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], kLog2e, -mc));
+        p[t][i] = (full || (vis >> i & 1)) ? e : 0.f;
+        sum += p[t][i];
+      }
+      l[t] += sum;
+    }
+    if (slow) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) masked_pv(b, p[t], acc[t], k0, lo[t], hi[t]);
+      return;
+    }
+    if constexpr (kBf16) {
+      // P in bf16 for the matrix product (as esgpt_attn_fwd and esgpt_attn_decode round it; the sums stay f32)
+      bf16x8 pf[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pf[t][i] = (__bf16)p[t][i];
+      const __bf16* vr = vt + (4 * g + (c >> 2)) * LD + 4 * (c & 3);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        typedef __attribute__((address_space(3))) bf16x4* lds4;
+        const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * d));
+        const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * LD + 16 * d));
+        bf16x8 vf;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          vf[i] = x[i];
+          vf[4 + i] = y[i];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], acc[t][d], 0, 0, 0);
+      }
+    } else {
+      const float* v = reinterpret_cast<const float*>(b.v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[(e * KD + (d >> 1)) * 2 + (d & 1)], p[t][e], acc[t][d],
+                                                             0, 0, 0);
+    }
+  }
+
+  // Page ids of the next 64 / KT blocks of this wave, one lane each; -1: past the end or not a page.
+  __device__ __forceinline__ int pages(const int32_t* tab, int k0, int stride, int k_end) {
+    const int key = k0 + (lane / KT) * stride + (lane % KT) * 16;
+    if (key >= k_end) return -1;
+    const int id = tab[key >> a.psl];
+    if (id >= 0 && id < a.n_pages) return id;
+    set_err(a.err, ESGPT_FLAG_BAD_PAGE);
+    return -1;
+  }
+
+  // Blocks k_first, k_first + stride, ... below k_end of the rows named by tab. k_first is a multiple of 16.
+  __device__ __forceinline__ void walk(const int32_t* tab, int k_first, int stride, int k_end, const int (&lo)[NT],
+                                       const int (&hi)[NT], const bool (&act)[NT]) {
+    int lo_all = 0, hi_all = 0x7fffffff;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      if (act[t]) {
+        lo_all = max(lo_all, lo[t]);
+        hi_all = min(hi_all, hi[t]);
+      }
+    lo_all = wave_max_i(lo_all);
+    hi_all = wave_min_i(hi_all);
+    if (k_first >= k_end) return;
+    constexpr int PER = 64 / KT;
+    int pid = pages(tab, k_first, stride, k_end), slot = 0;
+    Block b, nx;
+    load(b, k_first, k_end, pid, 0);
+    for (int k0 = k_first; k0 < k_end; k0 += stride) {
+      const int k1 = k0 + stride;
+      if (k1 < k_end) {
+        if (++slot == PER) {
+          slot = 0;
+          pid = pages(tab, k1, stride, k_end);
+        }
+        load(nx, k1, k_end, pid, slot);
+      }
+      bool full = k0 >= lo_all && k0 + KB <= hi_all && k0 + KB <= k_end;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) full = full && b.ok[t];
+      step(b, k0, lo, hi, full);
+      if (k1 < k_end) b = nx;
+    }
+  }
+};
+
+// v / l, zeros for a row that saw no key (l == 0; what v holds then does not count).
+template <typename T>
+__device__ __forceinline__ void store4(T* o, float4 v, float l) {
+  const bool none = l == 0.f;
+  const float inv = 1.f / l;
+  struct alignas(4 * sizeof(T)) Four { T e[4]; } x;
+  x.e[0] = from_f32<T>(none ? 0.f : v.x * inv);
+  x.e[1] = from_f32<T>(none ? 0.f : v.y * inv);
+  x.e[2] = from_f32<T>(none ? 0.f : v.z * inv);
+  x.e[3] = from_f32<T>(none ? 0.f : v.w * inv);
+  *reinterpret_cast<Four*>(o) = x;
+}
+
+// A part's result of one row: stored for the join, or, as the only part, divided and written to o.
+template <typename T>
+__device__ __forceinline__ void emit4(const SharedArgs& a, int64_t out, int h, int part, int d, float4 v, float m, float l,
+                                      bool first) {
+  const int64_t rh = out * a.H + h;
+  if (a.NP == 1) {
+    store4(reinterpret_cast<T*>(a.o) + rh * a.hd + d, v, l);
+    return;
+  }
+  const int64_t at = rh * a.NP + part;
+  if (first) *reinterpret_cast<float2*>(a.ml + 2 * at) = make_float2(m, l);
+  if (l != 0.f) *reinterpret_cast<float4*>(a.po + at * a.hd + d) = v;  // l == 0: the join does not read it
+}
+
+// The four waves' states of column tile t, joined per row through LDS: row r0 + i of the group (i < 16).
+template <typename T, int KD, int t, typename W>
+__device__ __forceinline__ void join_waves(const SharedArgs& a, const W& x, bool act, char* lds, int64_t out0, int r0,
+                                           int h, int ch) {
+  constexpr int OLD = KD * 32 + 4;
+  const int w = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, c = lane & 15;
+  float* jo = reinterpret_cast<float*>(lds);  // [wave][16][OLD]
+  float* jm = jo + kWaves * 16 * OLD;         // [wave][16]
+  float* jl = jm + kWaves * 16;
+  __syncthreads();  // the waves' V tiles, or the tile before
+  const float lw = act ? xsum(x.l[t]) : 0.f;
+  if (g == 0) {
+    jm[w * 16 + c] = x.m[t];
+    jl[w * 16 + c] = lw;
+  }
+#pragma unroll
+  for (int d = 0; d < W::DT; ++d) {
+    int dim;
+    const float4 v = four<T, W::DT>(x.acc[t], d, g, dim);
+    *reinterpret_cast<float4*>(jo + (w * 16 + c) * OLD + dim) = v;
+  }
+  __syncthreads();
+  const int row = threadIdx.x >> 4;
+  if (r0 + row >= a.M) return;
+  float M = -INFINITY, L = 0.f, f[kWaves];
+#pragma unroll
+  for (int u = 0; u < kWaves; ++u) M = fmaxf(M, jl[u * 16 + row] == 0.f ? -INFINITY : jm[u * 16 + row]);
+  const float mc = M == -INFINITY ? 0.f : M * kLog2e;
+#pragma unroll
+  for (int u = 0; u < kWaves; ++u) {
+    const float lu = jl[u * 16 + row];
+    f[u] = __builtin_amdgcn_exp2f(fmaf(jm[u * 16 + row], kLog2e, -mc));
+    if (lu != 0.f) L = fmaf(lu, f[u], L);
+  }
+  for (int d = 4 * (threadIdx.x & 15); d < a.hd; d += 64) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) {
+      if (jl[u * 16 + row] == 0.f) continue;  // this wave saw nothing for the row
+      const float4 y = *reinterpret_cast<const float4*>(jo + (u * 16 + row) * OLD + d);
+      v.x = fmaf(y.x, f[u], v.x);
+      v.y = fmaf(y.y, f[u], v.y);
+      v.z = fmaf(y.z, f[u], v.z);
+      v.w = fmaf(y.w, f[u], v.w);
+    }
+    emit4<T>(a, out0 + r0 + row, h, ch, d, v, M, L, d == 0);
+  }
+}
+
+template <typename T, int KD, int NT>
+__global__ __launch_bounds__(64 * kWaves) void shared_kernel(SharedArgs a) {
+  using W = Walk<T, KD, NT>;
+  constexpr int OLD = KD * 32 + 4;
+  constexpr int kTile = W::kBf16 ? W::KB * W::LD * 2 : 0;
+  constexpr int kJoin = kWaves * 16 * (OLD + 2) * 4;
+  __shared__ __align__(16) char lds[(kWaves * kTile > kJoin) ? kWaves * kTile : kJoin];
+  const int w = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, c = lane & 15;
+
+  if ((int)blockIdx.x >= a.units) {
+    // own rows of one (trajectory, head, chunk) per wave: column c is its new event c
+    const int64_t id = (int64_t)(blockIdx.x - a.units) * kWaves + w;
+    const int ch = (int)(id % a.NSc), h = (int)(id / a.NSc % a.H), s = (int)(id / a.NSc / a.H);
+    if (s >= a.S) return;
+    using W1 = Walk<T, KD, 1>;
+    W1 x(a, h, lds + w * kTile);
+    const Row r = row_of(a, s, c, c < a.Lq);
+    x.load_q(0, r);
+    const int hi = r.active ? min(r.at + 1, a.cap) : 0, lo = (r.active && a.window) ? max(0, r.at - a.window + 1) : 0;
+    const int base = wave_min_i(r.active ? lo : 0x7fffffff) & ~15;  // no active row: no key
+    const int end = wave_max_i(hi);
+    const int64_t first = (int64_t)base + (int64_t)ch * a.schunk;
+    const int los[1] = {lo}, his[1] = {hi};
+    const bool act[1] = {r.active};
+    if (first < end)
+      x.walk(a.table + (int64_t)s * a.table_w, (int)first, W1::KB, (int)min((int64_t)end, first + a.schunk), los, his, act);
+    const float l = r.active ? xsum(x.l[0]) : 0.f;
+    if (c < a.Lq) {
+      const int64_t out = (int64_t)s * a.Lq + c;
+#pragma unroll
+      for (int d = 0; d < W1::DT; ++d) {
+        int dim;
+        const float4 v = four<T, W1::DT>(x.acc[0], d, g, dim);
+        if (dim < a.hd) emit4<T>(a, out, h, a.NPc + ch, dim, v, x.m[0], l, d == 0 && g == 0);
+      }
+    }
+    return;
+  }
+
+  // history chunk of one (group, head, 16 NT rows): neighbouring workgroups of one XCD share a chunk's keys and values
+  const int id = xcd_linear(blockIdx.x, a.units);
+  const int rt = id % a.RT, ch = id / a.RT % a.NPc, gh = id / a.RT / a.NPc;
+  const int h = gh % a.H, grp = gh / a.H;
+  W x(a, h, lds + w * kTile);
+  const int P = prefix_len(a, grp);
+  int lo[NT], hi[NT], base = 0x7fffffff;
+  bool act[NT];
+  Row rows[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int rr = rt * 16 * NT + 16 * t + c;
+    rows[t] = row_of(a, grp * a.n + rr / a.Lq, rr % a.Lq, rr < a.M);
+    x.load_q(t, rows[t]);
+    act[t] = rows[t].active;
+    hi[t] = act[t] ? P : 0;
+    lo[t] = (act[t] && a.window) ? min(P, max(0, P + rows[t].at - a.window + 1)) : 0;
+    if (act[t]) base = min(base, lo[t]);
+  }
+  // chunks count from the first row that a window of this group can reach, whatever its own rows
+  const int from = (a.window ? max(0, P - a.window) : 0) & ~15;
+  const int64_t c0 = (int64_t)from + (int64_t)ch * a.pchunk;
+  const int64_t end = min((int64_t)P, c0 + a.pchunk);
+  base = wave_min_i(base) & ~15;
+  int64_t first = c0 + (int64_t)w * W::KB;
+  if (base > c0) {  // whole rounds of blocks before the first visible key
+    const int64_t skip = (base - c0) / (kWaves * W::KB) * (kWaves * W::KB);
+    first += skip;
+  }
+  if (first < end)
+    x.walk(a.prefix_table + (int64_t)grp * a.prefix_w, (int)first, kWaves * W::KB, (int)end, lo, hi, act);
+
+  const int64_t out0 = (int64_t)grp * a.M;
+  join_waves<T, KD, 0>(a, x, act[0], lds, out0, rt * 16 * NT, h, ch);
+  if constexpr (NT == 2) join_waves<T, KD, 1>(a, x, act[1], lds, out0, rt * 16 * NT + 16, h, ch);
+}
+
+// Joins a row's parts: o = sum_p e^{m_p - M} O_p / sum_p e^{m_p - M} l_p. One wave per (row, head): lane groups of
+// `width` lanes (4 dimensions each) take every (64 / width)-th part.
+template <typename T>
+__global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a, int64_t rows, int width) {
+  const int64_t rh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (rh >= rows) return;
+  const int lane = lane_id(), sub = lane / width, d = 4 * (lane % width), nsub = 64 / width;
+  const float2* ml = reinterpret_cast<const float2*>(a.ml) + rh * a.NP;
+  const float2 own = lane < a.NP ? ml[lane] : make_float2(-INFINITY, 0.f);  // NP <= 64
+  const float M = wave_max(own.y == 0.f ? -INFINITY : own.x);
+  const float mc = M == -INFINITY ? 0.f : M * kLog2e;
+  const float f = own.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(fmaf(own.x, kLog2e, -mc));
+  const float L = wave_sum(own.y == 0.f ? 0.f : own.y * f);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < a.NP; p0 += nsub) {
+    const int p = p0 + sub;
+    const float fp = __shfl(f, p & 63, 64), lp = __shfl(own.y, p & 63, 64);
+    if (p < a.NP && lp != 0.f && d < a.hd) {
+      const float4 y = *reinterpret_cast<const float4*>(a.po + (rh * a.NP + p) * a.hd + d);
+      v.x = fmaf(y.x, fp, v.x);
+      v.y = fmaf(y.y, fp, v.y);
+      v.z = fmaf(y.z, fp, v.z);
+      v.w = fmaf(y.w, fp, v.w);
+    }
+  }
+  for (int o = width; o < 64; o <<= 1) {
+    v.x += __shfl_xor(v.x, o, 64);
+    v.y += __shfl_xor(v.y, o, 64);
+    v.z += __shfl_xor(v.z, o, 64);
+    v.w += __shfl_xor(v.w, o, 64);
+  }
+  if (sub == 0 && d < a.hd) {
+    store4(reinterpret_cast<T*>(a.o) + rh * a.hd + d, v, L);
+  }
+}
+
+struct SharedPlan {
+  int NT, RT, NPc, NSc, NP, pchunk, schunk;
+  int64_t units, own_blocks;
+};
+
+SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t prefix_cap, int64_t cap, int64_t window,
+                       int dtype) {
+  SharedPlan p;
+  const int64_t M = (S / G) * Lq, kb = dtype == ESGPT_BF16 ? 32 : 16;
+  p.NT = dtype == ESGPT_BF16 && M > 16 ? 2 : 1;
+  p.RT = (int)cdiv(M, 16 * p.NT);
+  const int64_t round = kWaves * kb;
+  const int64_t pspan = window ? std::min(prefix_cap, window + 16) : prefix_cap;
+  const int64_t base = G * H * p.RT;
+  p.NPc = pspan ? (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, base), cdiv(pspan, round), 48})) : 0;
+  p.pchunk = p.NPc ? (int)(cdiv(cdiv(pspan, p.NPc), round) * round) : 0;
+  p.NPc = p.NPc ? (int)cdiv(pspan, p.pchunk) : 0;
+  const int64_t sspan = window ? std::min(cap, window + Lq + 16) : cap;
+  p.NSc = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(4096, S * H), cdiv(sspan, 2 * kb), 16}));
+  p.schunk = (int)(cdiv(cdiv(sspan, p.NSc), kb) * kb);
+  p.NSc = (int)cdiv(sspan, p.schunk);
+  p.NP = p.NPc + p.NSc;
+  p.units = base * p.NPc;
+  p.own_blocks = cdiv(S * H * p.NSc, kWaves);
+  return p;
+}
+
+template <typename T>
+int launch_shared(const SharedPlan& p, const SharedArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(p.units + p.own_blocks)), block(64 * kWaves);
+  const int kd = (a.hd + 31) / 32;
+#define SHARED(KD)                                                                        \
+  do {                                                                                    \
+    if constexpr (sizeof(T) == 2) {                                                       \
+      if (p.NT == 2) {                                                                    \
+        shared_kernel<T, KD, 2><<<grid, block, 0, st>>>(a);                               \
+        break;                                                                            \
+      }                                                                                   \
+    }                                                                                     \
+    shared_kernel<T, KD, 1><<<grid, block, 0, st>>>(a);                                   \
+  } while (0)
+  if (kd == 1) SHARED(1);
+  else if (kd == 2) SHARED(2);
+  else if (kd == 3) SHARED(3);
+  else SHARED(4);
+#undef SHARED
+  ESGPT_LAUNCH_CHECK();
+  if (p.NP > 1) {
+    int width = 1;
+    while (4 * width < a.hd) width *= 2;
+    const int64_t rows = (int64_t)a.S * a.Lq * a.H;
+    shared_join_kernel<T><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(a, rows, width);
+    ESGPT_LAUNCH_CHECK();
+  }
+  return ESGPT_OK;
+}
+
+bool shared_ok(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap, int64_t cap, int64_t window,
+               int dtype) {
+  return G > 0 && S >= G && S % G == 0 && Lq >= 1 && Lq <= kMaxLq && H > 0 && hd > 0 && hd <= 128 &&
+         hd % (dtype == ESGPT_BF16 ? 8 : 4) == 0 && (dtype == ESGPT_F32 || dtype == ESGPT_BF16) && prefix_cap >= 0 &&
+         cap >= 1 && prefix_cap <= (int64_t)1 << 29 && cap <= (int64_t)1 << 29 && window >= 0 &&
+         S * Lq * H < (int64_t)1 << 28;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t esgpt_attn_decode_shared_workspace(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap,
+                                          int64_t cap, int64_t window, int dtype) {
+  if (!shared_ok(G, S, Lq, H, hd, prefix_cap, cap, window, dtype)) return 0;
+  const SharedPlan p = shared_plan(G, S, Lq, H, prefix_cap, cap, std::min<int64_t>(window, (int64_t)1 << 30), dtype);
+  return p.NP > 1 ? (size_t)(S * Lq * H * p.NP) * (2 + hd) * sizeof(float) : 0;
+}
+
+int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_pages, int64_t n_pages,
+                             int64_t page_size, const int32_t* prefix_table, int64_t prefix_w,
+                             const int32_t* prefix_lens, int64_t G, const int32_t* page_table, int64_t table_w,
+                             const int32_t* past, const uint8_t* row_mask, void* o, int64_t S, int64_t Lq, int64_t H,
+                             int64_t hd, int64_t prefix_cap, int64_t cap, int64_t window, int dtype, void* workspace,
+                             size_t workspace_bytes, int32_t* err, void* stream) {
+  if (S == 0 && Lq >= 0 && Lq <= kMaxLq) return ESGPT_OK;
+  ESGPT_REQUIRE(shared_ok(G, S, Lq, H, hd, prefix_cap, cap, window, dtype));
+  ESGPT_REQUIRE(page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0 && n_pages >= 0 &&
+                n_pages < (int64_t)1 << 31 && cap <= table_w * page_size && prefix_cap <= prefix_w * page_size);
+  auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+  ESGPT_REQUIRE(q && o && past && page_table && aligned(q) && aligned(o) && (prefix_cap == 0 || (prefix_table && prefix_lens)));
+  ESGPT_REQUIRE(n_pages == 0 || (k_pages && v_pages && aligned(k_pages) && aligned(v_pages)));
+  window = std::min<int64_t>(window, (int64_t)1 << 30);
+  const SharedPlan p = shared_plan(G, S, Lq, H, prefix_cap, cap, window, dtype);
+  ESGPT_REQUIRE(p.units + p.own_blocks < (int64_t)1 << 31);
+  SharedArgs a{};
+  if (p.NP > 1) {
+    const size_t rows = (size_t)(S * Lq * H * p.NP);
+    ESGPT_REQUIRE(workspace && aligned(workspace) && workspace_bytes >= rows * (2 + hd) * sizeof(float));
+    a.po = reinterpret_cast<float*>(workspace);
+    a.ml = a.po + rows * hd;
+  }
+  a.q = q;
+  a.kp = k_pages;
+  a.vp = v_pages;
+  a.o = o;
+  a.prefix_table = prefix_table;
+  a.prefix_lens = prefix_lens;
+  a.table = page_table;
+  a.past = past;
+  a.row_mask = row_mask;
+  a.err = err;
+  a.n_pages = n_pages;
+  a.prefix_w = prefix_w;
+  a.table_w = table_w;
+  a.S = (int)S;
+  a.n = (int)(S / G);
+  a.Lq = (int)Lq;
+  a.H = (int)H;
+  a.hd = (int)hd;
+  a.psl = 0;
+  while ((1 << a.psl) < page_size) ++a.psl;
+  a.prefix_cap = (int)prefix_cap;
+  a.cap = (int)cap;
+  a.window = (int)window;
+  a.M = (int)((S / G) * Lq);
+  a.RT = p.RT;
+  a.NPc = p.NPc;
+  a.NSc = p.NSc;
+  a.NP = p.NP;
+  a.pchunk = p.pchunk;
+  a.schunk = p.schunk;
+  a.units = (int)p.units;
+  if (dtype == ESGPT_F32) return launch_shared<float>(p, a, as_stream(stream));
+  return launch_shared<bf16>(p, a, as_stream(stream));
+}
+
+}  // extern "C"

@@ -638,6 +638,51 @@ Tensor kv_append_paged(const Tensor& qkv_, const Tensor& k_pages, const Tensor& 
   return q;
 }
 
+Tensor attn_decode_shared(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages,
+                          const optional<Tensor>& prefix_table, const optional<Tensor>& prefix_lens,
+                          const Tensor& page_table, const Tensor& past, const optional<Tensor>& row_mask,
+                          int64_t prefix_cap, int64_t cap, int64_t window, const Tensor& err) {
+  const char* what = "esgpt.attn_decode_shared";
+  check_pages(what, q_, k_pages, v_pages);
+  const int64_t H = k_pages.size(1), ps = k_pages.size(2), hd = k_pages.size(3);
+  TORCH_CHECK(q_.dim() == 3 && q_.size(2) == H * hd, what, ": q must be [sequences, new events, ", H * hd, "]");
+  const int64_t S = q_.size(0), Lq = q_.size(1);
+  TORCH_CHECK(Lq <= 16, what, ": ", Lq, " new events a call, at most 16 (a longer run is a prompt: esgpt.attention)");
+  const c10::DeviceGuard guard(q_.device());
+  const bool pre = prefix_table.has_value() && prefix_table->defined();
+  TORCH_CHECK(pre == (prefix_lens.has_value() && prefix_lens->defined()) && (pre || prefix_cap == 0), what,
+              ": prefix_table and prefix_lens are given together, or not at all with prefix_cap = 0");
+  const int64_t G = pre ? prefix_table->size(0) : S;
+  if (pre) {
+    check_i32(what, "prefix_table", *prefix_table, q_, 2, G);
+    check_i32(what, "prefix_lens", *prefix_lens, q_, 1, G);
+    TORCH_CHECK(G > 0 ? S % G == 0 : S == 0, what, ": ", S, " sequences do not divide into ", G, " groups");
+    TORCH_CHECK(prefix_cap >= 0 && prefix_cap <= prefix_table->size(1) * ps, what, ": prefix_cap = ", prefix_cap,
+                " is beyond the ", prefix_table->size(1) * ps, " rows of prefix_table");
+  }
+  check_i32(what, "page_table", page_table, q_, 2, S);
+  check_i32(what, "past", past, q_, 1, S);
+  TORCH_CHECK(cap >= 1 && cap <= page_table.size(1) * ps, what, ": cap = ", cap, " is not within the ",
+              page_table.size(1) * ps, " rows of page_table");
+  TORCH_CHECK(window >= 0, what, ": window = ", window);
+  Tensor m = row_mask_of(what, row_mask, q_, S, Lq);
+  int32_t* e = err_of(what, err, q_);
+  Tensor q = rows16(q_);
+  Tensor o = at::empty({S, Lq, H * hd}, q.options());
+  if (o.numel() == 0) return o;
+  const int dt = dtype_code(q.scalar_type());
+  const size_t nb = esgpt_attn_decode_shared_workspace(G, S, Lq, H, hd, prefix_cap, cap, window, dt);
+  Tensor ws = at::empty({(int64_t)nb}, q.options().dtype(at::kByte));
+  check(esgpt_attn_decode_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.size(0), ps,
+                                 pre ? ptr<const int32_t>(*prefix_table) : nullptr, pre ? prefix_table->size(1) : 0,
+                                 pre ? ptr<const int32_t>(*prefix_lens) : nullptr, G, ptr<const int32_t>(page_table),
+                                 page_table.size(1), ptr<const int32_t>(past),
+                                 m.defined() ? ptr<const uint8_t>(m) : nullptr, o.data_ptr(), S, Lq, H, hd, prefix_cap,
+                                 cap, window, dt, ws.data_ptr(), nb, e, stream_of(q)),
+        "attn_decode_shared");
+  return o;
+}
+
 // ---- output-layer losses -------------------------------------------------------------------------------------------
 std::vector<esgpt_loss_term> make_terms(at::IntArrayRef t) {
   TORCH_CHECK(t.size() % 8 == 0, "terms: 8 ints per term");
@@ -1232,6 +1277,8 @@ TORCH_LIBRARY(esgpt, m) {
         "float eps) -> (Tensor, Tensor)");
   m.def("kv_append_paged(Tensor qkv, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor past, "
         "Tensor? row_mask, Tensor? q_w, Tensor? k_w, Tensor? pos, Tensor? inv_freq, float eps, Tensor err) -> Tensor");
+  m.def("attn_decode_shared(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? prefix_table, Tensor? prefix_lens, "
+        "Tensor page_table, Tensor past, Tensor? row_mask, int prefix_cap, int cap, int window, Tensor err) -> Tensor");
   m.def("output_loss(Tensor zc, Tensor? zt, Tensor? zc_bias, " BATCH_SCHEMA ", int n_levels, int shift, int[] terms, "
         "int[] tte_i, float[] tte_f, Tensor err, int path=0) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("residual_ln(Tensor? x, Tensor? y, Tensor? bias, Tensor ln_w, Tensor ln_b, Tensor? row_mask, float p, "
@@ -1296,6 +1343,7 @@ TORCH_LIBRARY_IMPL(esgpt, CUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
   m.impl("kv_append_paged", &kv_append_paged);
+  m.impl("attn_decode_shared", &attn_decode_shared);
   m.impl("output_loss", &output_loss);
   m.impl("residual_ln", &residual_ln);
   m.impl("residual_ln_bwd", &residual_ln_bwd);

@@ -646,6 +646,35 @@ def cached_attention(qkv: torch.Tensor, layer_past, key_mask: torch.Tensor | Non
 
 
 # ----------------------------------------------------------------------------------------------------------------
+# Generation: paged cache with a shared history (csrc/rope.hip, csrc/decode_shared.hip)
+# ----------------------------------------------------------------------------------------------------------------
+class PagedKV:
+    """One layer's pool of cache pages for ``esgpt::kv_append_paged`` and ``esgpt::attn_decode_shared``: ``k`` / ``v``
+    [n_pages, H, page_size, head size], and the list of free pages. ``pages(count)`` hands out page ids (one row of a
+    page table, int32 on the device) and ``release(ids)`` takes them back; which sequence a page belongs to, and how
+    many of its rows are filled, is the caller's (page tables and ``past`` are plain tensors)."""
+
+    def __init__(self, n_pages: int, page_size: int, H: int, head_size: int, dtype, device):
+        if page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
+            raise ValueError(f"page size {page_size} is not a power of two from 16 to 65536")
+        self.k = torch.empty(n_pages, H, page_size, head_size, dtype=dtype, device=device)
+        self.v = torch.empty_like(self.k)
+        self._free = list(range(n_pages))[::-1]
+
+    def pages(self, count: int) -> torch.Tensor:
+        if count > len(self._free):
+            raise RuntimeError(f"eventstreamgpt_amd: {count} cache pages asked for, {len(self._free)} of "
+                               f"{self.k.shape[0]} are free")
+        return torch.tensor([self._free.pop() for _ in range(count)], dtype=torch.int32, device=self.k.device)
+
+    def release(self, ids: torch.Tensor) -> None:
+        ids = [int(i) for i in ids.tolist()]
+        if len(set(ids)) != len(ids) or not all(0 <= i < self.k.shape[0] for i in ids) or set(ids) & set(self._free):
+            raise ValueError(f"pages {ids} are not handed out (each once)")
+        self._free.extend(ids)
+
+
+# ----------------------------------------------------------------------------------------------------------------
 # Output-layer losses
 # ----------------------------------------------------------------------------------------------------------------
 def terms_list(terms) -> list[int]:

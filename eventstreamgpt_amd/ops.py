@@ -33,7 +33,8 @@ Used by the NA glue's autograd Functions (transformer/structured_attention.py): 
 Non-differentiable: ``embed_bag_bwd``, ``embed_epilogue_bwd``, ``attention_bwd``, ``residual_ln_bwd``,
 ``bias_act_bwd``, ``qk_norm_rope_bwd``, ``linear_act``, ``linear_bwd`` (+ ``weight_grad_join``: with ``dw_tickets`` the weight gradient
 runs on a second stream, joined by that op), ``gemm`` / ``gemm_``, ``column_sum``, ``kv_append``,
-``attn_decode`` (generation), ``kv_append_paged`` (the same norm and rotation into a paged cache), ``pack`` (the compute-dtype parameter copies) and ``adamw``
+``attn_decode`` (generation), ``kv_append_paged`` (the same norm and rotation into a paged cache),
+``attn_decode_shared`` (attention over it, a history shared by several trajectories read once), ``pack`` (the compute-dtype parameter copies) and ``adamw``
 (generative_modeling.py:460-485).
 
 There is no CPU kernel: calling an operator on CPU tensors raises (no fallback).
@@ -52,7 +53,8 @@ ACT_DERIV = 8  # ESGPT_ACT_DERIV (include/esgpt_amd.h): the pre-activation buffe
 _state = {"loaded": False}
 
 OPS = ("embed_joint", "embed_split_bags", "embed_epilogue", "embed_epilogue_bwd", "embed_bag_bwd", "attention",
-       "attention_bwd", "kv_append", "attn_decode", "qk_norm_rope", "qk_norm_rope_bwd", "kv_append_paged", "output_loss", "residual_ln", "residual_ln_bwd", "bias_act",
+       "attention_bwd", "kv_append", "attn_decode", "qk_norm_rope", "qk_norm_rope_bwd", "kv_append_paged",
+       "attn_decode_shared", "output_loss", "residual_ln", "residual_ln_bwd", "bias_act",
        "bias_act_bwd", "column_sum", "gemm", "gemm_", "linear_act", "linear_bwd", "linear", "mlp", "head_loss",
        "pack", "adamw", "adamw_dev", "weight_grad_join", "residual_ln_bwd_partials", "colsum_flush", "seed_bank", "residual",
        "residual_bwd", "na_split", "na_split_bwd_", "na_assemble", "na_assemble_bwd", "na_head_split",
@@ -253,6 +255,10 @@ def _register():
     @fake(lib + "kv_append_paged")
     def _(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err):
         return qkv.new_empty(qkv.shape[0], qkv.shape[1], qkv.shape[2] // 3)
+
+    @fake(lib + "attn_decode_shared")
+    def _(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, past, row_mask, prefix_cap, cap, window, err):
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
 
     def _loss_fake(zc, zt, shift, n_terms, B):
         f32 = torch.float32

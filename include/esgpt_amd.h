@@ -259,6 +259,26 @@ int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, c
                           int64_t page_size, void* q, int64_t S, int64_t Lq, int64_t H, int64_t hd, int dtype,
                           int32_t* err, void* stream);
 
+/* esgpt_attn_decode_shared: attention of S sequences' Lq (1..16) new events over the paged cache, where the S / G
+ * sequences g*S/G .. of group g continue one history that is stored once (prefix pages) and read once for all of them:
+ *   o[s, i] = softmax_j(q[s, i] . k_j) v_j over the group's prefix_lens[g] history rows and the sequence's own rows
+ *   t <= past[s] + (rows before i that row_mask keeps), both in index order, window > 0: index distance < window.
+ * q [S, Lq, D] and the new events' own rows as esgpt_kv_append_paged left them (the same past and row_mask); o
+ * [S, Lq, D]: zeros in padded rows. prefix_table int32 [G, prefix_w] / page_table int32 [S, table_w] name pages of one
+ * pool. prefix_cap / cap: bounds on the prefix lengths and on past + new that the work is split by (at most the tables'
+ * room; prefix_cap = 0: no history, prefix_table / prefix_lens may be NULL); a length beyond its bound, a negative one
+ * or a page outside the pool raises ESGPT_FLAG_BAD_PAGE, and what lies there counts as not visible. Rows beyond a length
+ * are never read. A row whose visible scores are all -inf gives zeros. workspace: esgpt_attn_decode_shared_workspace
+ * bytes (0: none needed). */
+size_t esgpt_attn_decode_shared_workspace(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap,
+                                          int64_t cap, int64_t window, int dtype);
+int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_pages, int64_t n_pages,
+                             int64_t page_size, const int32_t* prefix_table, int64_t prefix_w,
+                             const int32_t* prefix_lens, int64_t G, const int32_t* page_table, int64_t table_w,
+                             const int32_t* past, const uint8_t* row_mask, void* o, int64_t S, int64_t Lq, int64_t H,
+                             int64_t hd, int64_t prefix_cap, int64_t cap, int64_t window, int dtype, void* workspace,
+                             size_t workspace_bytes, int32_t* err, void* stream);
+
 /* ---- Output layer losses -----------------------------------------------------------------------------------
  * GenerativeOutputLayerBase.get_{classification,regression,TTE}_outputs (model_output.py:1311-1721) with
  * weighted_loss / safe_weighted_avg (utils.py:134-234), fused: one pass computes every per-event loss, the

@@ -1,0 +1,550 @@
+"""Attention over a paged cache with a shared history (``esgpt::attn_decode_shared``) against a plain implementation in
+64 bits, alone and together with the operators that fill the cache.
+
+Tolerances, from u = 2^-24: a score is a chain of hd products and additions, off by (hd + 8) u of its terms'
+sizes, and a probability by twice that (its own and the normaliser's) + 16 u; the sum over n keys adds (n / 16 + 64) u
+(16 or 32 keys enter each accumulation). All of it relative to sum_j p_j |v_j|. With bf16 data P is rounded for the
+matrix product, half a step (2^-8) of each term, and so is the result.
+"""
+import math
+
+import pytest
+import torch
+
+U = 2.0**-24
+gpu = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def ops():
+    from eventstreamgpt_amd import ops as O
+
+    return O.load()
+
+
+def err():
+    from eventstreamgpt_amd import kernels as K
+
+    return K.err_word(torch.device(DEV, torch.cuda.current_device()))
+
+
+@pytest.fixture(autouse=True)
+def _clear(request):
+    on = request.node.get_closest_marker("gpu") is not None
+    if on:
+        err().zero_()
+    yield
+    if on:
+        err().zero_()
+
+
+class Case:
+    """Pools, tables and lengths on the CPU (``dev`` moves them), queries [G n, Lq, H hd]."""
+
+    def __init__(self, G, n, Lq, H, hd, ps, P, s, window=0, dt=F32, seed=0, ragged=True, share=False, masked=False):
+        g = torch.Generator().manual_seed(seed)
+        S = G * n
+        self.G, self.n, self.S, self.Lq, self.H, self.hd, self.ps, self.window, self.dt = G, n, S, Lq, H, hd, ps, window, dt
+        pp, sp = -(-P // ps), -(-s // ps)
+        pages = (pp + sp if share else G * pp + S * sp) + 2
+        at = torch.randperm(pages, generator=g).int()
+        if share:  # every group reads the same pages, and so does every sequence
+            self.prefix_table = at[:pp].repeat(G, 1)
+            self.table = at[pp: pp + sp].repeat(S, 1)
+        else:
+            self.prefix_table, self.table = at[: G * pp].view(G, pp), at[G * pp: G * pp + S * sp].view(S, sp)
+        self.prefix_lens = torch.randint(P // 2 if ragged else P, P + 1, (G,), generator=g).int()
+        self.past = torch.randint(0 if ragged else s - Lq, s - Lq + 1, (S,), generator=g).int()
+        self.row_mask = torch.rand(S, Lq, generator=g) < 0.6 if masked else None
+        std = 1.3 * hd**-0.25
+        self.q = (std * torch.randn(S, Lq, H * hd, generator=g)).to(dt)
+        self.kp = (std * torch.randn(pages, H, ps, hd, generator=g)).to(dt)
+        self.vp = torch.randn(pages, H, ps, hd, generator=g).to(dt)
+        self.P, self.s = P, s
+
+    def own_row(self, s, i):
+        return int(self.past[s]) + (i if self.row_mask is None else int(self.row_mask[s, :i].sum()))
+
+    def run(self, **kw):
+        d = dict(q=self.q, k_pages=self.kp, v_pages=self.vp, prefix_table=self.prefix_table if self.P else None,
+                 prefix_lens=self.prefix_lens if self.P else None, page_table=self.table, past=self.past,
+                 row_mask=self.row_mask, prefix_cap=self.P, cap=self.s, window=self.window)
+        d.update(kw)
+        d = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+        d.setdefault("err", err())
+        return ops().attn_decode_shared(**d)
+
+    def rows(self, pool, table, lo, hi):
+        """Rows lo .. hi - 1 named by one table row, [hi - lo, H, hd], in 64 bits; bad pages leave no rows: their
+        places are returned too."""
+        j = torch.arange(lo, hi)
+        page = table.long()[j // self.ps] if hi > lo else j
+        ok = (page >= 0) & (page < pool.shape[0])
+        return pool[page.clamp(0, max(pool.shape[0] - 1, 0)), :, j % self.ps].double(), ok
+
+    def oracle(self):
+        """(o, sum_j p_j |v_j|, largest sum_d |q_d k_d| of a row, keys of a row), [S, Lq, H, hd] or broadcastable."""
+        o = torch.zeros(self.S, self.Lq, self.H, self.hd, dtype=torch.float64)
+        mag, size = torch.zeros_like(o), torch.zeros(self.S, self.Lq, self.H, 1, dtype=torch.float64)
+        for s in range(self.S):
+            gr = s // self.n
+            P = min(max(int(self.prefix_lens[gr]), 0), self.P) if self.P else 0
+            for i in range(self.Lq):
+                if self.row_mask is not None and not bool(self.row_mask[s, i]) or int(self.past[s]) < 0:
+                    continue
+                at = self.own_row(s, i)
+                lo_p = max(0, P + at - self.window + 1) if self.window else 0
+                lo_s = max(0, at - self.window + 1) if self.window else 0
+                hi_s = min(at + 1, self.s)
+                parts = []
+                if min(lo_p, P) < P:
+                    parts.append((self.prefix_table[gr], lo_p, P))
+                if lo_s < hi_s:
+                    parts.append((self.table[s], lo_s, hi_s))
+                ks, vs = [], []
+                for tab, lo, hi in parts:
+                    k, ok = self.rows(self.kp, tab, lo, hi)
+                    v, _ = self.rows(self.vp, tab, lo, hi)
+                    ks.append(k[ok])
+                    vs.append(v[ok])
+                if not ks or sum(k.shape[0] for k in ks) == 0:
+                    continue
+                k, v = torch.cat(ks), torch.cat(vs)
+                q = self.q[s, i].double().view(1, self.H, self.hd)
+                p = torch.softmax((q * k).sum(-1), 0)[..., None]
+                o[s, i], mag[s, i] = (p * v).sum(0), (p * v.abs()).sum(0)
+                size[s, i, :, 0] = (q * k).abs().sum(-1).amax(0)
+        return o, mag, size
+
+    def check(self, got, want=None):
+        o, mag, size = want or self.oracle()
+        got = got.cpu().double().view(self.S, self.Lq, self.H, self.hd)
+        n = self.P + self.s
+        rel = 2 * (self.hd + 8) * U * size + (16 + n / 16 + 64) * U
+        lim = (rel + (2.0**-8 if self.dt == BF16 else 0)) * mag + (2.0**-8 if self.dt == BF16 else U) * o.abs()
+        bad = ~((got - o).abs() <= lim)
+        assert not bad.any(), (bad.sum().item(), (got - o).abs().max().item(), ((got - o).abs() / lim.clamp_min(1e-30)).max().item())
+
+
+CASES = [
+    # G, n, Lq, H, hd, ps, P, s, window
+    (1, 1, 1, 1, 8, 16, 1, 1, 0),        # the smallest call: one history row, one own row
+    (1, 4, 1, 4, 16, 16, 40, 6, 0), (2, 3, 1, 2, 24, 16, 0, 19, 0),  # no history at all
+    (3, 5, 1, 4, 64, 64, 77, 33, 0), (2, 16, 1, 2, 32, 32, 130, 64, 0),
+    (2, 17, 1, 2, 64, 64, 300, 20, 0),   # a row tile of one row
+    (1, 40, 1, 2, 96, 32, 201, 9, 0), (2, 3, 1, 3, 128, 16, 99, 40, 0), (1, 33, 1, 1, 128, 128, 640, 5, 0),
+    (2, 4, 3, 2, 64, 32, 70, 21, 0), (1, 9, 16, 2, 40, 16, 50, 31, 0), (2, 2, 2, 2, 16, 16, 17, 2, 0),
+    (2, 4, 1, 2, 64, 64, 300, 40, 32),   # the window reaches from the own rows into the history
+    (2, 20, 1, 2, 64, 64, 150, 90, 64), (2, 4, 4, 2, 32, 16, 40, 30, 5), (1, 3, 2, 1, 64, 16, 33, 18, 1),
+    (2, 3, 1, 2, 64, 64, 90, 20, 100000),
+    (1, 6, 1, 2, 64, 64, 9001, 700, 0),  # many parts of a row
+    (1, 2, 1, 1, 64, 16, 500, 3000, 0), (1, 40, 2, 1, 64, 64, 5000, 40, 700),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", CASES, ids=str)
+def test_against_the_oracle(c, dt):
+    x = Case(*c, dt=dt)
+    x.check(x.run())
+    assert int(err()[0]) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", [(64, 1, 1, 16, 16, 64, 4500, 3, 0), (300, 1, 1, 16, 16, 64, 3, 1300, 0),
+                               (64, 20, 1, 16, 16, 32, 4200, 2, 0)], ids=str)
+def test_more_keys_in_a_part_than_a_round_of_page_ids(c, dt):
+    """Enough workgroups that a history (or own) part is longer than 64 page ids reach; all sequences name the same
+    pages. The first sequences and the last one are checked."""
+    x = Case(*c, dt=dt, share=True)
+    got = x.run()
+    keep = sorted({0, 1, x.S // 2, x.S - 1})
+    G, n = x.G, x.n
+    sub = Case(*c, dt=dt, share=True)
+    for s in keep:
+        sub.S, sub.G, sub.n = 1, 1, 1
+        sub.prefix_table, sub.prefix_lens = x.prefix_table[s // n: s // n + 1], x.prefix_lens[s // n: s // n + 1]
+        sub.table, sub.past, sub.q = x.table[s: s + 1], x.past[s: s + 1], x.q[s: s + 1]
+        sub.check(got[s: s + 1])
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", [(2, 5, 4, 2, 64, 16, 50, 20, 0), (2, 9, 3, 2, 32, 16, 60, 30, 7), (3, 4, 1, 2, 64, 16, 20, 9, 0)],
+                         ids=str)
+def test_padded_rows(c, dt):
+    """Rows that row_mask drops are zeros; a sequence with none left gives zeros; the others see the same keys as ever."""
+    x = Case(*c, dt=dt, masked=True)
+    x.row_mask[0] = False
+    got = x.run()
+    x.check(got)
+    assert (got[~x.row_mask.to(DEV)] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf, "lowest"])
+def test_what_lies_beyond_a_length_never_counts(dt, junk):
+    """Unused rows of used pages and unused pages hold NaN, infinities or the type's lowest value."""
+    junk = torch.finfo(dt).min if junk == "lowest" else junk
+    for c in [(2, 5, 1, 2, 64, 64, 70, 21, 0), (2, 3, 3, 2, 24, 16, 30, 12, 9), (1, 18, 1, 2, 96, 32, 45, 33, 0)]:
+        x = Case(*c, dt=dt)
+        want = x.oracle()
+        clean = x.run()
+        used = torch.zeros(x.kp.shape[0], x.ps, dtype=torch.bool)
+        for gr in range(x.G):
+            for j in range(int(x.prefix_lens[gr])):
+                used[x.prefix_table[gr, j // x.ps], j % x.ps] = True
+        for s in range(x.S):
+            for j in range(x.own_row(s, x.Lq - 1) + 1):
+                used[x.table[s, j // x.ps], j % x.ps] = True
+        m = ~used[:, None, :, None]
+        x.kp.masked_fill_(m, junk)
+        x.vp.masked_fill_(m, junk)
+        got = x.run()
+        assert torch.equal(got, clean)
+        x.check(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("junk", [math.nan, math.inf])
+def test_not_finite_values_reach_only_the_rows_that_see_them(dt, junk):
+    """A value that is not finite at a key which some rows of a tile see and others do not (a window's edge in the
+    history, a later new event, another trajectory's own row)."""
+    x = Case(1, 6, 3, 2, 64, 16, 60, 14, window=20, dt=dt, ragged=True, seed=3)
+    clean = x.run().view(x.S, x.Lq, x.H, x.hd)
+    want = x.oracle()
+    P = int(x.prefix_lens[0])
+    kill = torch.zeros(x.S, x.Lq, x.H, x.hd, dtype=torch.bool)
+    # one history row near the windows' edges, dimension 5 of head 1; one row of sequence 2, dimension 40 of head 0
+    j = P - 12
+    x.vp[x.prefix_table[0, j // 16], 1, j % 16, 5] = junk
+    t = x.own_row(2, 1)
+    x.vp[x.table[2, t // 16], 0, t % 16, 40] = junk
+    for s in range(x.S):
+        for i in range(x.Lq):
+            if P + x.own_row(s, i) - j < x.window:
+                kill[s, i, 1, 5] = True
+    kill[2, 1:, 0, 40] = True
+    assert kill[:, :, 1, 5].any() and not kill[:, :, 1, 5].all()
+    got = x.run().view(x.S, x.Lq, x.H, x.hd)
+    assert not torch.isfinite(got.cpu()[kill]).any()
+    ok = ~kill
+    o, mag, size = want
+    x.check(torch.where(kill.to(DEV), clean, got), want)
+    assert torch.isfinite(got.cpu()[ok]).all()
+    # a key that is not finite makes the rows that see it NaN and no other
+    x.kp[x.table[4, x.own_row(4, 2) // 16], 0, x.own_row(4, 2) % 16, 3] = math.nan
+    got = x.run().view(x.S, x.Lq, x.H, x.hd)
+    assert got[4, 2, 0].isnan().all() and torch.isfinite(got[4, :2, 0].cpu()).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+def test_large_scores(dt):
+    """Scores of several hundred, one key far above the rest, all keys equal: the running maximum carries them."""
+    for c in [(1, 4, 1, 2, 64, 16, 200, 20, 0), (1, 20, 1, 2, 64, 64, 900, 20, 0)]:
+        x = Case(*c, dt=dt)
+        x.q *= 40
+        x.check(x.run())
+        x = Case(*c, dt=dt)
+        x.kp[x.prefix_table[0, 3], :, 7] *= 30
+        x.check(x.run())
+        x.kp.fill_(0.25)
+        x.check(x.run())
+
+
+@gpu
+def test_bad_pages_and_lengths_are_flagged_and_not_read():
+    from eventstreamgpt_amd import kernels as K
+
+    for spoil in ("page", "own_page", "prefix_len", "prefix_len_negative", "past", "past_negative"):
+        x = Case(2, 3, 2, 2, 32, 16, 64, 32, ragged=False)
+        x.check(x.run())
+        K.check_errors()
+        if spoil == "page":
+            x.prefix_table[0, 1], x.prefix_table[1, 2] = x.kp.shape[0], -5
+        elif spoil == "own_page":
+            x.table[1, 0], x.table[4, 1] = 2**31 - 1, -(2**31)
+        elif spoil == "prefix_len":
+            x.prefix_lens[1] = 2**31 - 1
+        elif spoil == "prefix_len_negative":
+            x.prefix_lens[0] = -7
+        elif spoil == "past":
+            x.past[2] = 2**31 - 1
+        else:
+            x.past[3] = -1
+        got = x.run()
+        if spoil == "past":  # all of the table's rows are visible, no more
+            x.past[2] = x.s - 1
+        x.check(got)
+        with pytest.raises(IndexError, match="paged cache"):
+            K.check_errors()
+        K.check_errors()
+    x = Case(2, 3, 1, 2, 32, 16, 64, 32)
+    got = x.run(k_pages=x.kp[:0], v_pages=x.vp[:0])
+    assert (got == 0).all()
+    with pytest.raises(IndexError):
+        K.check_errors()
+
+
+@gpu
+def test_bounds_wider_than_the_lengths():
+    """Caps far above the lengths (a cache with room to grow) change the split, not the result beyond rounding."""
+    for dt in (F32, BF16):
+        x = Case(2, 3, 1, 2, 64, 16, 400, 300, dt=dt)
+        x.prefix_lens, x.past = torch.tensor([3, 0]).int(), torch.tensor([0, 1, 2, 0, 17, 299]).int()
+        want = x.oracle()
+        x.check(x.run(), want)
+        x.P, x.s = 400, 300
+        x.check(x.run(prefix_cap=x.prefix_table.shape[1] * 16, cap=x.table.shape[1] * 16), want)
+
+
+@gpu
+def test_layouts_streams_and_repeats():
+    x = Case(2, 9, 2, 4, 64, 64, 700, 50, dt=BF16)
+    want = x.run()
+    D = x.H * x.hd
+    wide = torch.zeros(x.S, x.Lq, 3 * D, dtype=BF16, device=DEV)
+    wide[..., :D] = x.q.to(DEV)
+    odd = torch.zeros(x.q.numel() + 1, dtype=BF16, device=DEV)
+    odd[1:] = x.q.reshape(-1).to(DEV)
+    for q in (wide[..., :D], odd[1:].view(x.q.shape)):
+        assert torch.equal(x.run(q=q), want)
+    st = torch.cuda.Stream()
+    q, e = x.q.to(DEV), err()
+    st.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        got = x.run(q=q, err=e)
+    here = x.run()  # at the same time on this stream: workspaces are the calls' own
+    st.synchronize()
+    assert torch.equal(got, want) and torch.equal(here, want)
+
+
+@gpu
+def test_captured_generation_steps():
+    """One graph with an append and the attention; each replay takes the next event (past grows on the device), with
+    eager work on the same cache layout in between."""
+    x = Case(2, 4, 1, 2, 64, 16, 100, 48, dt=BF16, ragged=False)
+    D = x.H * x.hd
+    d = {k: getattr(x, k).to(DEV) for k in ("prefix_table", "prefix_lens", "table", "kp", "vp")}
+    past = torch.zeros(x.S, dtype=torch.int32, device=DEV)
+    qkv = torch.zeros(x.S, 1, 3 * D, dtype=BF16, device=DEV)
+    pos = torch.zeros(x.S, 1, device=DEV)
+    f = torch.exp(-torch.arange(32, device=DEV) / 8).float()
+    w = torch.full((64,), 64**-0.25, device=DEV)
+
+    def step(kp, vp):
+        q = ops().kv_append_paged(qkv, kp, vp, d["table"], past, None, w, w, pos, f, 1e-6, err())
+        return ops().attn_decode_shared(q, kp, vp, d["prefix_table"], d["prefix_lens"], d["table"], past, None, 100, 48, 0,
+                                        err())
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        step(d["kp"].clone(), d["vp"].clone())
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(d["kp"], d["vp"])
+    kp, vp = d["kp"].clone(), d["vp"].clone()
+    g = torch.Generator().manual_seed(1)
+    for i in range(20):
+        qkv.copy_(torch.randn(qkv.shape, generator=g).to(BF16))
+        pos.add_(37.5)
+        graph.replay()
+        eager = step(kp, vp)
+        past.add_(1)
+        torch.cuda.synchronize()
+        assert torch.equal(held, eager) and torch.equal(kp, d["kp"]) and torch.equal(vp, d["vp"]), i
+    assert int(err()[0]) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 24])
+def test_prompt_then_generation(dt, window):
+    """As a model layer runs them: the left-padded histories are normalised, rotated and attended with esgpt::attention
+    and stored once; four trajectories of each continue event by event. Every new event's output equals causal
+    attention over the whole sequence (history and own events) in 64 bits, and esgpt::attention's last row on it."""
+    from eventstreamgpt_amd import kernels as K
+
+    B, L, n, T, H, hd, ps = 3, 37, 4, 9, 4, 64, 16
+    D, S = H * hd, B * n
+    g = torch.Generator().manual_seed(2)
+    pads = torch.tensor([0, 11, 30])
+    mask = (torch.arange(L)[None] >= pads[:, None]).to(DEV)
+    w = [(hd**-0.25 * (1 + 0.2 * torch.randn(hd, generator=g))).to(DEV) for _ in range(2)]
+    f = torch.exp(torch.arange(0, hd, 2) * (-math.log(10000.0) / hd)).float().to(DEV)
+    hist = torch.randn(B, L, 3 * D, generator=g).to(dt).to(DEV)
+    t_hist = torch.exp(3 + torch.randn(B, L, generator=g)).cumsum(1).to(DEV)
+    new = torch.randn(S, T, 3 * D, generator=g).to(dt).to(DEV)
+    t_new = (t_hist[:, -1:].repeat_interleave(n, 0).cpu() + torch.exp(3 + torch.randn(S, T, generator=g)).cumsum(1)).to(DEV)
+
+    cache = K.PagedKV(64, ps, H, hd, dt, DEV)
+    prefix_table = torch.stack([cache.pages(-(-L // ps)) for _ in range(B)])
+    table = torch.stack([cache.pages(-(-T // ps)) for _ in range(S)])
+    zero = torch.zeros(B, dtype=torch.int32, device=DEV)
+    ops().kv_append_paged(hist, cache.k, cache.v, prefix_table, zero, mask, *w, t_hist, f, 1e-6, err())
+    prefix_lens = mask.sum(1).int()
+    past = torch.zeros(S, dtype=torch.int32, device=DEV)
+    whole = torch.cat([hist.repeat_interleave(n, 0), new], 1)
+    times = torch.cat([t_hist.repeat_interleave(n, 0), t_new], 1)
+    keys = torch.cat([mask.repeat_interleave(n, 0), torch.ones(S, T, dtype=torch.bool, device=DEV)], 1)
+    y = ops().qk_norm_rope(whole, *w, times, f, H, 1e-6)
+    for i in range(T):
+        q = ops().kv_append_paged(new[:, i: i + 1].contiguous(), cache.k, cache.v, table, past, None, *w, t_new[:, i: i + 1],
+                                  f, 1e-6, err())
+        o = ops().attn_decode_shared(q, cache.k, cache.v, prefix_table, prefix_lens, table, past, None, L, T, window, err())
+        past += 1
+        end = L + i + 1
+        yq, yk, yv = y[:, :end].double().view(S, end, 3, H, hd).unbind(2)
+        assert torch.equal(q[:, 0], y[:, end - 1, :D])
+        sc = (yq[:, -1:] * yk).sum(-1)
+        far = torch.arange(end, device=DEV)
+        # index distance counts stored events: left padding is not stored, so it is the plain distance
+        see = keys[:, :end] & ((end - 1 - far < window) if window else torch.ones_like(far, dtype=torch.bool))
+        p = torch.softmax(sc.masked_fill(~see[..., None], -math.inf), 1)[..., None]
+        want, mag = (p * yv).sum(1).reshape(S, D), (p * yv.abs()).sum(1).reshape(S, D)
+        size = (yq[:, -1:] * yk).abs().sum(-1).amax().item()
+        lim = (2 * (hd + 8) * U * size + 96 * U + (2.0**-8 if dt == BF16 else 0)) * mag + (2.0**-8 if dt == BF16 else U) * want.abs()
+        assert ((o[:, 0].double() - want).abs() <= lim).all(), i
+        ref, _, _ = ops().attention(y[:, :end].contiguous(), keys[:, :end].contiguous(), None, H, window, False, 0.0, None)
+        assert ((ref[:, -1].double() - want).abs() <= 4 * lim + 1e-5).all(), i
+    K.check_errors()
+
+
+@gpu
+def test_without_a_history_it_is_the_dense_cache_attention():
+    """Paged rows of unequal lengths against esgpt::attn_decode over a dense copy, f32: two f32 results, each within
+    its bound of the same number."""
+    x = Case(5, 1, 1, 4, 32, 16, 0, 60)
+    got = x.run()
+    D = x.H * x.hd
+    for s in range(x.S):
+        Lk = int(x.past[s]) + 1
+        k, v = (torch.stack([p[x.table[s, j // 16], :, j % 16] for j in range(Lk)]).reshape(1, Lk, D) for p in (x.kp, x.vp))
+        qkv = torch.cat([x.q[s: s + 1], k[:, -1:], v[:, -1:]], -1).to(DEV)
+        ref = ops().attn_decode(qkv, k.contiguous().to(DEV), v.contiguous().to(DEV), None, None, x.H, Lk, 0)
+        assert (got[s] - ref[0]).abs().max() <= 2e-5
+    x.check(got)
+
+
+@gpu
+def test_pools_beyond_32_bit_offsets():
+    """Pages of 2 MiB whose elements lie past 2^31 (5 GiB pools): stored and read at their place."""
+    H, hd, ps, pages = 8, 128, 1024, 2300
+    kp, vp = (torch.empty(pages, H, ps, hd, dtype=BF16, device=DEV) for _ in range(2))
+    for at in (kp, vp):
+        at[0].zero_()
+        at[-3:].zero_()
+    x = Case(1, 2, 1, H, hd, 16, 20, 40, dt=BF16)
+    table = torch.tensor([[pages - 1], [pages - 2]], dtype=torch.int32, device=DEV)
+    pre = torch.tensor([[pages - 3]], dtype=torch.int32, device=DEV)
+    g = torch.Generator().manual_seed(0)
+    for tab, S, L in ((pre, 1, 20), (table, 2, 33)):
+        rows = torch.randn(S, L, 3 * H * hd, generator=g).to(BF16).to(DEV)
+        ops().kv_append_paged(rows, kp, vp, tab, torch.zeros(S, dtype=torch.int32, device=DEV), None, None, None, None, None,
+                              1e-6, err())
+        for s in range(S):
+            assert torch.equal(kp[tab[s, 0], :, :L].transpose(0, 1).reshape(L, -1), rows[s, :, H * hd: 2 * H * hd])
+    q = (0.1 * torch.randn(2, 1, H * hd, generator=g)).to(BF16)
+    args = (torch.tensor([20]).int().to(DEV), table, torch.tensor([32, 7]).int().to(DEV), None, 20, 33, 0, err())
+    big = ops().attn_decode_shared(q.to(DEV), kp, vp, pre, *args)
+    sk, sv = kp[-3:].clone(), vp[-3:].clone()
+    small = ops().attn_decode_shared(q.to(DEV), sk, sv, pre - (pages - 3), args[0], table - (pages - 3), *args[2:])
+    assert torch.equal(big, small) and torch.isfinite(big).all() and (big != 0).any()
+    assert (kp[0] == 0).all() and int(err()[0]) == 0
+
+
+@gpu
+def test_empty_calls():
+    x = Case(2, 3, 1, 2, 32, 16, 64, 32)
+    e = dict(q=x.q[:0], page_table=x.table[:0], past=x.past[:0], prefix_table=None, prefix_lens=None, prefix_cap=0)
+    assert x.run(**e).shape == (0, 1, 64)
+    assert x.run(q=x.q[:, :0]).shape == (6, 0, 64)
+
+
+@gpu
+def test_refusals():
+    x = Case(2, 3, 1, 2, 32, 16, 64, 32)
+    for kw, text in [
+        (dict(q=x.q[..., :32]), "q must be"), (dict(q=x.q[0]), "q must be"), (dict(q=x.q.bfloat16()), "pages must be"),
+        (dict(q=x.q.expand(6, 17, 64)), "at most 16"), (dict(prefix_table=None), "together"),
+        (dict(prefix_lens=None), "together"), (dict(prefix_table=None, prefix_lens=None), "together"),
+        (dict(prefix_table=x.prefix_table[:1].repeat(4, 1), prefix_lens=x.prefix_lens[:1].repeat(4)), "divide"),
+        (dict(prefix_lens=x.prefix_lens[:1]), "prefix_lens"), (dict(prefix_table=x.prefix_table.long()), "prefix_table"),
+        (dict(page_table=x.table[:3]), "page_table"), (dict(past=x.past.long()), "past"),
+        (dict(row_mask=torch.ones(6, 2).bool()), "row_mask"), (dict(prefix_cap=65), "prefix_cap"),
+        (dict(prefix_cap=-1), "prefix_cap"), (dict(cap=33), "cap"), (dict(cap=0), "cap"), (dict(window=-1), "window"),
+        (dict(k_pages=x.kp[:, :, ::2]), "k_pages and v_pages"), (dict(err=torch.zeros(2, dtype=torch.int64)), "error block"),
+    ]:
+        if "err" in kw:
+            with pytest.raises(RuntimeError, match=text):
+                ops().attn_decode_shared(x.q.to(DEV), x.kp.to(DEV), x.vp.to(DEV), None, None, x.table.to(DEV), x.past.to(DEV),
+                                         None, 0, 32, 0, kw["err"])
+            continue
+        with pytest.raises(RuntimeError, match=text):
+            x.run(**kw)
+
+
+# ------------------------------------------------------------------------------------------- without a device
+def test_c_abi_refuses_before_it_launches():
+    import os
+
+    from eventstreamgpt_amd import _lib as L
+
+    if not os.path.exists(L.LIB_PATH):
+        pytest.skip("library not built")
+    lib = L.load(require_device=False)
+    P = 4096
+
+    def call(q=P, kp=P, vp=P, n_pages=9, ps=64, pt=P, pw=4, pl=P, G=2, tab=P, tw=2, past=P, o=P, S=6, Lq=1, H=4, hd=64,
+             pcap=256, cap=128, window=0, dt=1, ws=P, nb=1 << 30):
+        return lib.esgpt_attn_decode_shared(q, kp, vp, n_pages, ps, pt, pw, pl, G, tab, tw, past, None, o, S, Lq, H, hd, pcap,
+                                            cap, window, dt, ws, nb, None, None)
+
+    for bad in (dict(q=None), dict(q=P + 8), dict(kp=None), dict(vp=P + 4), dict(n_pages=-1), dict(ps=8), dict(ps=96),
+                dict(ps=131072), dict(pt=None), dict(pl=None), dict(G=0), dict(G=4), dict(G=7), dict(tab=None), dict(past=None),
+                dict(o=None), dict(o=P + 2), dict(S=-1), dict(Lq=0), dict(Lq=17), dict(H=0), dict(hd=12), dict(hd=136), dict(hd=0),
+                dict(pcap=-1), dict(pcap=257), dict(cap=0), dict(cap=129), dict(window=-1), dict(dt=2), dict(ws=None),
+                dict(ws=P + 4), dict(nb=64), dict(S=1 << 27)):
+        assert call(**bad) == 1, bad
+    assert call(S=0) == 0
+    need = lib.esgpt_attn_decode_shared_workspace
+    assert need(2, 6, 1, 4, 64, 256, 128, 0, 1) > 0
+    assert need(6, 6, 1, 4, 64, 0, 16, 0, 1) == 0       # one part: written directly
+    assert need(2, 6, 17, 4, 64, 256, 128, 0, 1) == 0   # not a valid call
+
+
+def test_fake_tensors():
+    o = ops()
+    m = dict(device="meta", dtype=torch.int32)
+    kp = torch.empty(4, 2, 16, 32, device="meta")
+    q = torch.empty(3, 1, 64, device="meta")
+    out = o.attn_decode_shared(q, kp, kp, None, None, torch.empty(3, 1, **m), torch.empty(3, **m), None, 0, 16, 0,
+                               torch.empty(2, device="meta", dtype=torch.int64))
+    assert out.shape == q.shape
+
+
+def test_paged_cache_hands_out_each_page_once():
+    from eventstreamgpt_amd.kernels import PagedKV
+
+    c = PagedKV(6, 16, 2, 32, torch.float32, "cpu")
+    assert c.k.shape == (6, 2, 16, 32) and c.v.shape == c.k.shape and c.k.dtype == torch.float32
+    a, b = c.pages(2), c.pages(3)
+    assert a.dtype == torch.int32 and sorted(a.tolist() + b.tolist()) == sorted(set(a.tolist() + b.tolist()))
+    with pytest.raises(RuntimeError, match="1 of 6"):
+        c.pages(2)
+    c.release(a)
+    assert sorted(c.pages(3).tolist() + b.tolist()) == list(range(6))
+    with pytest.raises(ValueError, match="not handed out"):
+        c.release(torch.tensor([0, 0]))
+    for ps in (8, 24, 1 << 17):
+        with pytest.raises(ValueError, match="page size"):
+            PagedKV(2, ps, 2, 32, torch.float32, "cpu")
