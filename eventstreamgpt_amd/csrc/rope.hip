@@ -25,6 +25,7 @@ using namespace esgpt;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxRun = 512;      // tokens of a run
 constexpr int64_t kMaxD = 16384;  // H * hd: keeps the kernels' 32-bit divisions exact (fdiv)
 
 enum : int { MODE_FWD = 0, MODE_BWD = 1, MODE_APPEND = 2 };
@@ -41,7 +42,7 @@ struct RopeArgs {
   int64_t N;
   int pos_i64, R2, H, hd, C, GP, slots, passes, run;
   float eps;
-  uint64_t magic_r, magic_v;  // division by R2 and by a token's 16-B chunks of v
+  uint64_t magic_r;  // division by R2
   // append
   const uint8_t* row_mask;    // [S, Lq] or null
   const int32_t* past;        // [S]
@@ -50,7 +51,7 @@ struct RopeArgs {
   void* v_pages;
   int32_t* err;
   int64_t n_pages, table_w;
-  int Lq, ps;
+  int Lq, ps, psl;  // psl: log2 of the page size
 };
 
 __device__ __forceinline__ void turn_sincos(const RopeArgs& a, int64_t n, int i, float& s, float& c) {
@@ -92,33 +93,65 @@ __device__ __forceinline__ void st(T* p, const float (&v)[V]) {
   *reinterpret_cast<Chunk<T, V>*>(p) = c;
 }
 
-// Rows [0, i) of a sequence's mask that are set, by the whole workgroup (append: where the first token of the run
-// lands). `red`: one int per wave.
-__device__ __forceinline__ int mask_prefix(const uint8_t* m, int i, int* red) {
+// Rows [0, i) of a sequence's mask that are set, counted by this wave's share; the waves' counts go to red.
+__device__ __forceinline__ void mask_count(const uint8_t* m, int i, int* red) {
   int c = 0;
+#pragma unroll 4
   for (int j = threadIdx.x; j < i; j += blockDim.x) c += m[j] != 0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
-  if (lane_id() == 0) red[threadIdx.x >> 6] = c;
-  __syncthreads();
-  int t = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) t += red[w];
-  return t;
+  const float sum = wave_sum((float)c);  // below 2^24: exact
+  if (lane_id() == 0) red[threadIdx.x >> 6] = (int)sum;
 }
 
 // q = n / d for n, d < 2^16 by the host's magic = ceil(2^32 / d).
 __device__ __forceinline__ int fdiv(int n, uint64_t magic) { return (int)(((uint64_t)(uint32_t)n * magic) >> 32); }
 
+// Append: the element offset (head 0) of the cache row of each of the run's nt <= 64 tokens, one lane of the first wave
+// each; kMasked or kNowhere. A token's row counts the kept rows of its sequence before it: those before the run from
+// `red`, those in the run from the wave's ballot. What does not depend on the count is loaded before it (Token).
+struct Token {
+  int s, i;  // sequence, row of it
+  bool keep;
+  int past;
+};
+__device__ __forceinline__ Token token_of(const RopeArgs& a, int n, bool in) {
+  Token k{n / a.Lq, 0, in, 0};
+  k.i = n - k.s * a.Lq;
+  if (!in) return k;
+  k.past = a.past[k.s];
+  if (a.row_mask) k.keep = a.row_mask[n] != 0;
+  return k;
+}
+__device__ __forceinline__ int64_t place(const RopeArgs& a, const Token& k, const int* red, bool report) {
+  const int lane = lane_id();
+  int64_t row = k.i;
+  if (a.row_mask) {
+    uint64_t before = __ballot(k.keep) & (lane ? ~0ull >> (64 - lane) : 0ull);
+    if (lane > k.i) before &= ~0ull << (lane - k.i);  // the sequence began within the run: its own tokens only
+    row = __popcll(before);
+    if (lane <= k.i)
+      for (int w = 0; w < (int)(blockDim.x >> 6); ++w) row += red[w];
+  }
+  if (!k.keep) return kMasked;
+  row += k.past;
+  if (k.past >= 0 && row < a.table_w << a.psl) {
+    const int page = a.page_table[k.s * a.table_w + (row >> a.psl)];
+    if (page >= 0 && page < a.n_pages) return (((int64_t)page * a.H << a.psl) + (row & (a.ps - 1))) * a.hd;
+  }
+  if (report) set_err(a.err, ESGPT_FLAG_BAD_PAGE);
+  return kNowhere;
+}
+
 // blockDim.x = the slots * 2H * GP lanes of `slots` tokens, rounded up to whole waves (passes > 1: one token's
 // 2H * GP lanes in passes of 256). Run r of the grid-strided list of runs covers tokens [r * run, (r + 1) * run).
 template <typename T, int V, int MODE, bool NORM>
-__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(kThreads, MODE == MODE_BWD ? 4 : 1) void rope_kernel(RopeArgs a) {
   extern __shared__ __align__(16) char smem[];
   const int H = a.H, hd = a.hd, R2 = a.R2, D = H * hd, GP = a.GP;
   const int64_t ld_x = 3 * (int64_t)D;
   const int ipt = 2 * H * GP;  // lanes of one token
-  float2* cs = reinterpret_cast<float2*>(smem);                                            // [run][R2]
-  int64_t* dst = reinterpret_cast<int64_t*>(smem + (size_t)a.run * R2 * sizeof(float2));   // append: [run]
+  float* ws = reinterpret_cast<float*>(smem);                  // norm weights [2][hd]: in LDS, for the registers' sake
+  float2* cs = reinterpret_cast<float2*>(ws + 2 * hd);         // [run][R2], 8 entries at least
+  int64_t* dst = reinterpret_cast<int64_t*>(cs + max(a.run * R2, 8));  // append: [run]
   const int tid = threadIdx.x;
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* dy = reinterpret_cast<const T*>(a.dy);
@@ -137,19 +170,45 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
     const bool rot = e < R2;
     const int lo = rot ? e : e + R2;  // the chunk and its partner in the head
     const int hi = lo + (rot ? R2 : hd / 2 - R2);
-    const int64_t col = (int64_t)hh * hd;  // q heads, then k heads: contiguous in the packed row
-    float wl[V], wh[V], al[V], ah[V];      // weights; sums of dw
+    const int64_t col = live ? (int64_t)hh * hd : 0;  // q heads, then k heads: contiguous in the packed row
+    float al[V], ah[V];  // sums of dw
     if constexpr (NORM) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        wl[j] = on ? a.w[isk][lo + j] : 0.f;
-        wh[j] = on ? a.w[isk][hi + j] : 0.f;
-        al[j] = ah[j] = 0.f;
-      }
+      for (int j = 0; j < V; ++j) al[j] = ah[j] = 0.f;
+      for (int i = tid; i < 2 * hd; i += blockDim.x) ws[i] = a.w[i >= hd][i >= hd ? i - hd : i];
     }
+    const float* wt = ws + (live ? isk * hd : 0);
+    // v is copied 16 B a lane: a token's vch chunks are at most its lanes, and neighbours in both
+    constexpr int E = 16 / (int)sizeof(T);
+    const int vch = D / E;
+    const bool von = slot < a.slots && item < vch;
+    const int vh = item * E / hd;  // append: the chunk's head
+
     for (int64_t r = blockIdx.x; r < n_runs; r += gridDim.x) {
       const int64_t n0 = r * a.run;
       const int nt = (int)min((int64_t)a.run, a.N - n0);
+      Chunk<T, V> xl, xh, dl, dh;
+      uint4 vv;
+      // One token's loads, the same for every lane: one without a chunk of its own loads its group's first (or the
+      // token's first) and stores nothing.
+      auto fetch = [&](int64_t n) {
+        const T* xp = x + n * ld_x + col;
+        xl = ld<T, V>(xp + lo);
+        xh = ld<T, V>(xp + hi);
+        if constexpr (MODE == MODE_BWD) {
+          const T* dp = dy + n * ld_x + col;
+          dl = ld<T, V>(dp + lo);
+          dh = ld<T, V>(dp + hi);
+        }
+        if constexpr (MODE != MODE_BWD) vv = *reinterpret_cast<const uint4*>(x + n * ld_x + 2 * D + (von ? item * E : 0));
+      };
+      // the first token's loads are in flight while the run's sines and cosines (and cache rows) are worked out
+      Token tok;
+      if constexpr (MODE == MODE_APPEND) tok = token_of(a, (int)n0 + min(tid, nt - 1), tid < nt);
+      const int64_t n1 = min(n0 + slot, a.N - 1);
+      bool keep = MODE != MODE_BWD;
+      if constexpr (MODE == MODE_APPEND) keep = !a.row_mask || a.row_mask[n1] != 0;
+      if (keep) fetch(n1);
       __syncthreads();  // the previous run's readers of cs / dst
       for (int i = tid; i < nt * R2; i += blockDim.x) {
         const int t = fdiv(i, a.magic_r);
@@ -159,53 +218,48 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
       }
       if constexpr (MODE == MODE_APPEND) {
         int* red = reinterpret_cast<int*>(dst + a.run);
-        const int64_t s0 = n0 / a.Lq;
-        const int before = a.row_mask ? mask_prefix(a.row_mask + s0 * a.Lq, (int)(n0 - s0 * a.Lq), red) : 0;
-        for (int t = tid; t < nt; t += blockDim.x) {
-          const int64_t n = n0 + t, s = n / a.Lq;
-          int64_t d = kMasked;
-          if (!a.row_mask || a.row_mask[n]) {
-            int64_t row = n - s * a.Lq;
-            if (a.row_mask) {
-              row = s == s0 ? before : 0;
-              for (int64_t j = max(n0, s * a.Lq); j < n; ++j) row += a.row_mask[j] != 0;
-            }
-            const int64_t past = a.past[s];
-            row += past;
-            d = kNowhere;
-            if (past >= 0 && row < a.table_w * a.ps) {
-              const int64_t page = a.page_table[s * a.table_w + row / a.ps];
-              if (page >= 0 && page < a.n_pages) d = (page * H * a.ps + row % a.ps) * hd;
-            }
-            if (d == kNowhere && pass == 0) set_err(a.err, ESGPT_FLAG_BAD_PAGE);
-          }
-          dst[t] = d;
+        if (a.row_mask) {
+          const int i0 = (int)n0 % a.Lq;
+          mask_count(a.row_mask + n0 - i0, i0, red);
+          __syncthreads();
+        }
+        if (tid < 64) {
+          const int64_t d = place(a, tok, red, pass == 0);
+          if (tid < nt) dst[tid] = d;
         }
       }
       __syncthreads();
 
-      if (live) {
-        for (int t = slot; t < nt; t += a.slots) {
-          const int64_t n = n0 + t;
-          float fl[V], fh[V];
-          if (on) {
-            const T* xp = x + n * ld_x + col;
-            const Chunk<T, V> xl = ld<T, V>(xp + lo), xh = ld<T, V>(xp + hi);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              fl[j] = to_f32(xl.e[j]);
-              fh[j] = to_f32(xh.e[j]);
+      for (int t = slot; t < nt; t += a.slots) {
+        const int64_t n = n0 + t;
+        int64_t d = 0;
+        if constexpr (MODE == MODE_APPEND) {
+          d = dst[t];
+          if (d == kMasked) {  // padding: nothing is read, the query is zero
+            if (on && !isk) {
+              const float z[V] = {};
+              st<T, V>(out + n * D + col + lo, z);
+              st<T, V>(out + n * D + col + hi, z);
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) fl[j] = fh[j] = 0.f;
+            continue;
           }
-          float cn[V], sn[V];
+        }
+        if (MODE == MODE_BWD || t != slot) fetch(n);
+        if (von) {
+          if constexpr (MODE == MODE_APPEND) {
+            if (d >= 0)
+              *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_pages) + d + (int64_t)vh * a.ps * hd + (item * E - vh * hd)) = vv;
+          } else if constexpr (MODE == MODE_FWD) {
+            *reinterpret_cast<uint4*>(out + n * ld_x + 2 * D + item * E) = vv;
+          }
+        }
+        if (live) {
+          const float2* ct = cs + (rot ? t * R2 + e : 0);  // V entries are there for any lane, used where rot
+          float fl[V], fh[V], yl[V], yh[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const float2 v = rot && R2 > 0 ? cs[t * R2 + e + j] : make_float2(1.f, 0.f);
-            cn[j] = v.x;
-            sn[j] = v.y;
+            fl[j] = on ? to_f32(xl.e[j]) : 0.f;
+            fh[j] = on ? to_f32(xh.e[j]) : 0.f;
           }
           float rstd = 1.f;
           if constexpr (NORM) {
@@ -214,86 +268,60 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
             for (int j = 0; j < V; ++j) ss = fmaf(fl[j], fl[j], fmaf(fh[j], fh[j], ss));
             rstd = rsqrtf(fmaf(group_sum(ss, GP), inv_hd, a.eps));
           }
-          float yl[V], yh[V];
           if constexpr (MODE == MODE_BWD) {
-            float gl[V], gh[V];
-            if (on) {
-              const T* dp = dy + n * ld_x + col;
-              const Chunk<T, V> dl = ld<T, V>(dp + lo), dh = ld<T, V>(dp + hi);
+            float gx = 0.f;
 #pragma unroll
-              for (int j = 0; j < V; ++j) {
-                const float p = to_f32(dl.e[j]), q = to_f32(dh.e[j]);
-                gl[j] = rot ? fmaf(p, cn[j], q * sn[j]) : p;
-                gh[j] = rot ? fmaf(q, cn[j], -p * sn[j]) : q;
+            for (int j = 0; j < V; ++j) {
+              // a few LDS reads at a time: all of them at once do not fit 128 registers
+              if (V == 8 && j % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+              const float p = on ? to_f32(dl.e[j]) : 0.f, q = on ? to_f32(dh.e[j]) : 0.f;
+              const float2 v = ct[j];
+              yl[j] = rot ? fmaf(p, v.x, q * v.y) : p;
+              yh[j] = rot ? fmaf(q, v.x, -p * v.y) : q;
+              if constexpr (NORM) {
+                al[j] = fmaf(yl[j], fl[j] * rstd, al[j]);
+                ah[j] = fmaf(yh[j], fh[j] * rstd, ah[j]);
+                yl[j] *= wt[lo + j];
+                yh[j] *= wt[hi + j];
+                gx = fmaf(yl[j], fl[j], fmaf(yh[j], fh[j], gx));
               }
-            } else {
-#pragma unroll
-              for (int j = 0; j < V; ++j) gl[j] = gh[j] = 0.f;
             }
             if constexpr (NORM) {
-              float gx = 0.f;
-#pragma unroll
-              for (int j = 0; j < V; ++j) {
-                al[j] = fmaf(gl[j], fl[j] * rstd, al[j]);
-                ah[j] = fmaf(gh[j], fh[j] * rstd, ah[j]);
-                gl[j] *= wl[j];
-                gh[j] *= wh[j];
-                gx = fmaf(gl[j], fl[j], fmaf(gh[j], fh[j], gx));
-              }
               const float m = group_sum(gx, GP) * inv_hd * rstd * rstd;
 #pragma unroll
               for (int j = 0; j < V; ++j) {
-                gl[j] = rstd * (gl[j] - fl[j] * m);
-                gh[j] = rstd * (gh[j] - fh[j] * m);
+                yl[j] = rstd * (yl[j] - fl[j] * m);
+                yh[j] = rstd * (yh[j] - fh[j] * m);
               }
-            }
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              yl[j] = gl[j];
-              yh[j] = gh[j];
             }
           } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              const float p = NORM ? fl[j] * rstd * wl[j] : fl[j], q = NORM ? fh[j] * rstd * wh[j] : fh[j];
-              yl[j] = rot ? fmaf(p, cn[j], -q * sn[j]) : p;
-              yh[j] = rot ? fmaf(q, cn[j], p * sn[j]) : q;
+              const float p = NORM ? fl[j] * rstd * wt[lo + j] : fl[j], q = NORM ? fh[j] * rstd * wt[hi + j] : fh[j];
+              const float2 v = ct[j];
+              yl[j] = rot ? fmaf(p, v.x, -q * v.y) : p;
+              yh[j] = rot ? fmaf(q, v.x, p * v.y) : q;
             }
           }
-          if (!on) continue;
+          bool store = on;
           T* op = out + n * ld_x + col;
           if constexpr (MODE == MODE_APPEND) {
-            const int64_t d = dst[t];
             if (!isk) {
               op = out + n * D + col;
-              if (d == kMasked) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) yl[j] = yh[j] = 0.f;
-              }
             } else {
-              if (d < 0) continue;
+              store = store && d >= 0;
               op = reinterpret_cast<T*>(a.k_pages) + d + (int64_t)(hh - H) * a.ps * hd;
             }
           }
-          st<T, V>(op + lo, yl);
-          st<T, V>(op + hi, yh);
-        }
-      }
-      if (pass == 0) {  // v: copied, 16 B a lane
-        constexpr int E = 16 / (int)sizeof(T);
-        const int vch = D / E;
-        const T* vp = (MODE == MODE_BWD ? dy : x) + 2 * D;
-        for (int i = tid; i < nt * vch; i += blockDim.x) {
-          const int t = fdiv(i, a.magic_v), f = (i - t * vch) * E;
-          const uint4 v = *reinterpret_cast<const uint4*>(vp + (n0 + t) * ld_x + f);
-          if constexpr (MODE == MODE_APPEND) {
-            const int64_t d = dst[t];
-            if (d < 0) continue;
-            const int h = f / hd;
-            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_pages) + d + (int64_t)h * a.ps * hd + (f - h * hd)) = v;
-          } else {
-            *reinterpret_cast<uint4*>(out + (n0 + t) * ld_x + 2 * D + f) = v;
+          if (store) {
+            st<T, V>(op + lo, yl);
+            st<T, V>(op + hi, yh);
           }
+        }
+        if constexpr (MODE == MODE_BWD) {  // not among the token's first loads: no registers left to hold it
+          if (von)
+            *reinterpret_cast<uint4*>(out + n * ld_x + 2 * D + item * E) =
+                *reinterpret_cast<const uint4*>(dy + n * ld_x + 2 * D + item * E);
         }
       }
     }
@@ -338,6 +366,36 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
   }
 }
 
+// dw = the workgroups' partial sums, in a fixed order: 16 columns a workgroup, 64 interleaved groups of rows.
+__global__ __launch_bounds__(256) void dw_sum_kernel(const float* part, int64_t n, int width, float* dw) {
+  __shared__ float4 s[64][4];
+  const int c4 = threadIdx.x & 3, grp = threadIdx.x >> 2, col = blockIdx.x * 16 + 4 * c4;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < width) {
+#pragma unroll 8
+    for (int64_t r = grp; r < n; r += 64) {
+      const float4 v = *reinterpret_cast<const float4*>(part + r * width + col);
+      t.x += v.x;
+      t.y += v.y;
+      t.z += v.z;
+      t.w += v.w;
+    }
+  }
+  s[grp][c4] = t;
+  for (int h = 32; h > 0; h >>= 1) {
+    __syncthreads();
+    if (grp < h) {
+      const float4 v = s[grp + h][c4];
+      t.x += v.x;
+      t.y += v.y;
+      t.z += v.z;
+      t.w += v.w;
+      s[grp][c4] = t;
+    }
+  }
+  if (grp == 0 && col < width) *reinterpret_cast<float4*>(dw + col) = t;
+}
+
 struct Plan {
   int V, C, GP, slots, passes, block, run;
   int64_t grid;
@@ -346,7 +404,8 @@ struct Plan {
 
 // V: the widest access (up to 16 B) that the rotated half and half of what is not rotated are whole multiples of.
 // The workgroup takes as many tokens at once as give it up to 256 lanes, and one to four such sets per run: more
-// tokens per run cost fewer barriers and workgroups, while fewer keep the chip full (kRuns runs at least).
+// tokens per run cost fewer barriers and workgroups (and fewer chains of loads to find a token's cache row), while
+// fewer keep the chip full (kRuns runs at least).
 Plan make_plan(int64_t N, int64_t H, int64_t hd, int64_t R, int dtype, int mode) {
   Plan p;
   const int64_t R2 = R / 2, tail = hd / 2 - R2;
@@ -357,14 +416,15 @@ Plan make_plan(int64_t N, int64_t H, int64_t hd, int64_t R, int dtype, int mode)
   p.GP = 1;
   while (p.GP < p.C) p.GP *= 2;
   const int64_t ipt = 2 * H * p.GP;
+  const int64_t most = mode == MODE_APPEND ? 64 : kMaxRun;  // tokens of a run
   p.passes = (int)cdiv(ipt, kThreads);
-  p.slots = p.passes > 1 ? 1 : (int)(kThreads / ipt);
+  p.slots = p.passes > 1 ? 1 : (int)std::min<int64_t>(kThreads / ipt, most / 2);
   p.block = p.passes > 1 ? kThreads : (int)(cdiv(p.slots * ipt, 64) * 64);
-  const int64_t kRuns = mode == MODE_BWD ? 1024 : 2048;
-  const int64_t sets = std::max<int64_t>(1, std::min<int64_t>(4, N / (p.slots * kRuns)));
+  const int64_t kRuns = mode == MODE_FWD ? 2048 : 1024;
+  const int64_t sets = std::max<int64_t>(1, std::min<int64_t>({4, most / p.slots, N / (p.slots * kRuns)}));
   p.run = (int)(p.slots * sets);
   p.grid = std::min<int64_t>(cdiv(N, p.run), mode == MODE_BWD ? 1024 : (int64_t)1 << 20);
-  p.lds = (size_t)p.run * R2 * sizeof(float2);
+  p.lds = 2 * hd * sizeof(float) + std::max<size_t>((size_t)p.run * R2, 8) * sizeof(float2);  // 8: see ct in the kernel
   if (mode == MODE_APPEND) p.lds += (size_t)p.run * 8 + 4 * 4;
   if (mode == MODE_BWD) p.lds = std::max(p.lds, (size_t)p.block * 2 * V * sizeof(float));
   return p;
@@ -421,9 +481,7 @@ RopeArgs rope_args(const Plan& p, const void* x, const float* q_w, const float* 
   a.passes = p.passes;
   a.run = p.run;
   a.eps = eps;
-  const uint64_t vch = (uint64_t)(H * hd) / (dtype == ESGPT_BF16 ? 8 : 4);
   a.magic_r = R ? ((1ull << 32) + R / 2 - 1) / (R / 2) : 0;
-  a.magic_v = ((1ull << 32) + vch - 1) / vch;
   return a;
 }
 
@@ -473,8 +531,9 @@ int esgpt_qk_norm_rope_bwd(const void* dout, const void* qkv, const float* q_w, 
   launch<MODE_BWD>(p, a, dtype, st);
   ESGPT_LAUNCH_CHECK();
   if (!q_w) return ESGPT_OK;
-  const esgpt_colsum_job job{a.part, p.grid, 2 * hd, dw};
-  return esgpt_colsum_jobs(&job, 1, stream);
+  dw_sum_kernel<<<(unsigned)cdiv(2 * hd, 16), 256, 0, st>>>(a.part, p.grid, (int)(2 * hd), dw);
+  ESGPT_LAUNCH_CHECK();
+  return ESGPT_OK;
 }
 
 int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, const void* pos, int pos_dtype,
@@ -482,7 +541,8 @@ int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, c
                           const int32_t* page_table, int64_t table_w, void* k_pages, void* v_pages, int64_t n_pages,
                           int64_t page_size, void* q, int64_t S, int64_t Lq, int64_t H, int64_t hd, int dtype,
                           int32_t* err, void* stream) {
-  ESGPT_REQUIRE(S >= 0 && Lq >= 0 && Lq < (int64_t)1 << 31 && S < (int64_t)1 << 31);
+  constexpr int64_t kTop = ((int64_t)1 << 31) - 1024;  // the kernel counts tokens in 32 bits
+  ESGPT_REQUIRE(S >= 0 && Lq >= 0 && Lq <= kTop && S <= kTop && S * Lq <= kTop);
   ESGPT_REQUIRE(rope_ok(qkv, q_w, k_w, pos, pos_dtype, inv_freq, R, S * Lq, H, hd, eps, dtype));
   ESGPT_REQUIRE(page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0 && table_w >= 0 &&
                 n_pages >= 0);
@@ -502,6 +562,7 @@ int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, c
   a.table_w = table_w;
   a.Lq = (int)Lq;
   a.ps = (int)page_size;
+  while (((int64_t)1 << a.psl) < page_size) ++a.psl;
   launch<MODE_APPEND>(p, a, dtype, as_stream(stream));
   ESGPT_LAUNCH_CHECK();
   return ESGPT_OK;

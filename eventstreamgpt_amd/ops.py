@@ -4,7 +4,8 @@ The operators are defined and implemented in C++ (``csrc/torch_ops.cpp`` → ``l
 ``TORCH_LIBRARY(esgpt, m)`` with HIP implementations that call the C ABI of ``libesgpt_amd.so``). This module loads
 that library and registers, per operator, a fake (meta) kernel — output shapes / dtypes without running anything,
 for fake tensors, ``torch.compile`` and export — and, for the differentiable ones, the autograd formula
-(``torch.library.register_autograd``) whose backward calls the matching ``*_bwd`` operator.
+(``torch.library.register_autograd``; ``qk_norm_rope``: in ``csrc/torch_ops.cpp``) whose backward calls the matching
+``*_bwd`` operator.
 
 Differentiable operators and the reference code they replace:
 
@@ -468,23 +469,6 @@ def _register():
         return dqkv, None, None, None, None, None, None, None
 
     reg(lib + "attention", _at_bwd, setup_context=_at_setup)
-
-    # qk_norm_rope: d qkv from the raw buffer (the norms are recomputed), d q_w and d k_w summed in a fixed order
-    def _qr_setup(ctx, inputs, output):
-        qkv, q_w, k_w, pos, inv_freq, H, eps = inputs
-        if ctx.needs_input_grad[3] or ctx.needs_input_grad[4]:
-            raise NotImplementedError("eventstreamgpt_amd: qk_norm_rope has no gradient for pos and inv_freq")
-        ctx.save_for_backward(qkv, q_w, k_w, pos, inv_freq)
-        ctx.meta = (H, eps)
-
-    def _qr_bwd(ctx, dout):
-        H, eps = ctx.meta
-        qkv, q_w, k_w, pos, inv_freq = ctx.saved_tensors
-        dqkv, dw = ops.qk_norm_rope_bwd(dout, qkv, q_w, k_w, pos, inv_freq, H, eps)
-        dq_w, dk_w = (None, None) if q_w is None else (dw[0], dw[1])
-        return dqkv, dq_w, dk_w, None, None, None, None
-
-    reg(lib + "qk_norm_rope", _qr_bwd, setup_context=_qr_setup)
 
     # residual: d x (all rows of x; zeros for the rows skip_T leaves out), d y (y's dtype)
     def _rs_setup(ctx, inputs, output):
