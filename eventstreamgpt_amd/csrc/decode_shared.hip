@@ -128,27 +128,12 @@ __device__ __forceinline__ float4 four(const f32x4 (&acc)[DT], int d, int g, int
   }
 }
 
-template <typename T, int KD, int NT>
-struct Walk {
-  static constexpr bool kBf16 = sizeof(T) == 2;
-  static constexpr int KT = kBf16 ? 2 : 1;  // 16-key tiles per block: both types move 8 KB (hd 64) per block and wave
-  static constexpr int KB = 16 * KT;
-  static constexpr int DT = 2 * KD;      // 16-wide tiles of the head
-  static constexpr int LD = KD * 32 + 16;  // LDS row of V (elements): 8 mod 16 dwords, transposed reads hit all banks
-
-  const SharedArgs& a;
-  int h, lane, g, c;  // g = lane / 16, c = lane % 16
-  __bf16* vt;         // bf16: this wave's V tile, KB x LD
+// The online softmax of NT x 16 rows: O^T tiles (column = row of q), running maximum, this lane's share of the sum.
+template <int NT, int DT>
+struct State {
   f32x4 acc[NT][DT];
   float m[NT], l[NT];
-  uint4 qf[NT][kBf16 ? KD : 2 * KD];
-
-  __device__ __forceinline__ Walk(const SharedArgs& a_, int h_, void* lds) : a(a_), h(h_) {
-    lane = lane_id();
-    g = lane >> 4;
-    c = lane & 15;
-    vt = reinterpret_cast<__bf16*>(lds);
-    offsets();
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = -INFINITY;
@@ -157,32 +142,34 @@ struct Walk {
       for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
-  // Queries: column c of tile t is row `out` of q. bf16: chunk kd holds dims 32 kd + 8 g .. + 7; f32: chunk k holds
-  // dims 16 k + 4 g .. + 3 (the products contract over lane groups, in this permuted order on both sides).
-  __device__ __forceinline__ void load_q(int t, const Row& r) {
-    constexpr int NQ = kBf16 ? KD : 2 * KD, E = kBf16 ? 8 : 4;
-    const T* p = reinterpret_cast<const T*>(a.q) + (r.out * a.H + h) * a.hd;
-#pragma unroll
-    for (int k = 0; k < NQ; ++k) {
-      const int d = k * 4 * E + E * g;
-      qf[t][k] = (r.active && d < a.hd) ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
-    }
-  }
+};
 
-  static constexpr int NK = kBf16 ? KD : 2 * KD;        // 16-B chunks of a key that a lane holds
-  static constexpr int LPR = KD == 3 ? 16 : 4 * KD;      // bf16: lanes that read one row of V (12 of 16 at 96)
-  static constexpr int NV = kBf16 ? LPR / 2 : 2 * KD;    // bf16: 16-B loads of a block's V; f32: 16-B register groups
-
-  struct Block {
-    uint4 k[KT * NK], v[NV];
-    const T* vb[KT];  // first row of each tile's values
-    bool ok[KT];      // false: a bad page
-  };
-
-  // Byte offsets of this lane's chunks in a 16-row tile; beyond the head's width: out of every range (reads zero).
+// One wave's walk over blocks of keys.
+template <typename T, int KD>
+struct Walk {
+  static constexpr bool kBf16 = sizeof(T) == 2;
+  static constexpr int KT = kBf16 ? 2 : 1;  // 16-key tiles per block: both types move 8 KB (hd 64) per block and wave
+  static constexpr int KB = 16 * KT;
+  static constexpr int DT = 2 * KD;        // 16-wide tiles of the head
+  static constexpr int LD = KD * 32 + 16;  // LDS row of V (elements): 8 mod 16 dwords, transposed reads hit all banks
+  static constexpr int NK = kBf16 ? KD : 2 * KD;     // 16-B chunks of a key, or of a query, that a lane holds
+  static constexpr int LPR = KD == 3 ? 16 : 4 * KD;  // bf16: lanes that read one row of V (12 of 16 at 96)
+  static constexpr int NV = kBf16 ? LPR / 2 : 2 * KD;  // bf16: 16-B loads of a block's V; f32: 16-B register groups
+  static constexpr int PER = 64 / KT;                  // blocks whose page ids one load brings
   static constexpr int kOut = 1 << 30;
+  using Q = uint4[NK];
+
+  const SharedArgs& a;
+  int h, lane, g, c;  // g = lane / 16, c = lane % 16
+  __bf16* vt;         // bf16: this wave's V tile, KB x LD
+  // Byte offsets of this lane's chunks in a 16-row tile; beyond the head's width: out of every range (reads zero).
   int ko[NK], vo[kBf16 ? 1 : KD];
-  __device__ __forceinline__ void offsets() {
+
+  __device__ __forceinline__ Walk(const SharedArgs& a_, int h_, void* lds) : a(a_), h(h_) {
+    lane = lane_id();
+    g = lane >> 4;
+    c = lane & 15;
+    vt = reinterpret_cast<__bf16*>(lds);
     constexpr int E = kBf16 ? 8 : 4;
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
@@ -201,45 +188,84 @@ struct Walk {
     }
   }
 
-  // Loads the block at key k0 by range-checked buffer loads: zeros past k_end and on a bad page. pid: page ids of this
-  // round of blocks, lane slot * KT + tile.
-  __device__ __forceinline__ void load(Block& b, int k0, int k_end, int pid, int slot) {
-    const int rb = a.hd * (int)sizeof(T);
+  // Queries: column c is row `out` of q. bf16: chunk k holds dims 32 k + 8 g .. + 7; f32: dims 16 k + 4 g .. + 3 (the
+  // products contract over lane groups, in this permuted order on both sides).
+  __device__ __forceinline__ void load_q(Q& qf, const Row& r) const {
+    constexpr int E = kBf16 ? 8 : 4;
+    const T* p = reinterpret_cast<const T*>(a.q) + (r.out * a.H + h) * a.hd;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const int d = k * 4 * E + E * g;
+      qf[k] = (r.active && d < a.hd) ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  // Page ids of the 64 / KT blocks from k0 on, one lane each, for keys below `limit` (a bound that needs no length to
+  // have arrived); -1 beyond. check(): what the walk up to k_end uses of them.
+  __device__ __forceinline__ int key_of(int k0, int stride) const { return k0 + (lane / KT) * stride + (lane % KT) * 16; }
+  __device__ __forceinline__ int pages(const int32_t* tab, int k0, int stride, int limit) const {
+    const int key = key_of(k0, stride);
+    return k0 >= 0 && key < limit ? tab[key >> a.psl] : -1;
+  }
+  __device__ __forceinline__ int check(int id, int k0, int stride, int k_end) const {
+    if (key_of(k0, stride) >= k_end) return -1;
+    if (id >= 0 && id < a.n_pages) return id;
+    set_err(a.err, ESGPT_FLAG_BAD_PAGE);
+    return -1;
+  }
+
+  // A block's 16-row tiles in the pools: range-checked buffers that read zeros past k_end and on a bad page.
+  struct Tiles {
+    __amdgpu_buffer_rsrc_t k[KT], v[KT];
+    const T* vb[KT];
+    bool ok[KT];
+  };
+  __device__ __forceinline__ Tiles tiles(int k0, int k_end, int pid, int slot) const {
+    Tiles b;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       const int id = __builtin_amdgcn_readlane(pid, slot * KT + t);
       b.ok[t] = id >= 0;
       const int64_t row = b.ok[t] ? (((int64_t)id * a.H + h) << a.psl) + ((k0 + 16 * t) & ((1 << a.psl) - 1)) : 0;
-      const int n = b.ok[t] ? min(16, max(0, k_end - k0 - 16 * t)) * rb : 0;
-      const T* kb = reinterpret_cast<const T*>(a.kp) + row * a.hd;
+      const int n = b.ok[t] ? min(16, max(0, k_end - k0 - 16 * t)) * a.hd * (int)sizeof(T) : 0;
       b.vb[t] = reinterpret_cast<const T*>(a.vp) + row * a.hd;
-      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kb), (short)0, n, 0x00020000);
-      const __amdgpu_buffer_rsrc_t rv =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(b.vb[t]), (short)0, n, 0x00020000);
+      b.k[t] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(reinterpret_cast<const T*>(a.kp) + row * a.hd), (short)0,
+                                                 n, 0x00020000);
+      b.v[t] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(b.vb[t]), (short)0, n, 0x00020000);
+    }
+    return b;
+  }
+  __device__ __forceinline__ void load_k(uint4 (&k)[KT * NK], const Tiles& b) const {
 #pragma unroll
-      for (int k = 0; k < NK; ++k)
-        b.k[t * NK + k] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko[k], 0, 0));
-      if constexpr (kBf16) {
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+        k[t * NK + i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b.k[t], ko[i], 0, 0));
+  }
+  __device__ __forceinline__ void load_v(uint4 (&v)[NV], const Tiles& b) const {
+    const int rb = a.hd * (int)sizeof(T);
+    if constexpr (kBf16) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < NV / 2; ++i)
-          b.v[t * (NV / 2) + i] = __builtin_bit_cast(
-              uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, vo[0] + i * (64 / LPR) * rb, 0, 0));
-      } else {
-        float2* v = reinterpret_cast<float2*>(b.v);
+          v[t * (NV / 2) + i] = __builtin_bit_cast(
+              uint4, __builtin_amdgcn_raw_buffer_load_b128(b.v[t], vo[0] + i * (64 / LPR) * rb, 0, 0));
+    } else {
+      float2* f = reinterpret_cast<float2*>(v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int p = 0; p < KD; ++p)
-            v[e * KD + p] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rv, vo[p] + e * rb, 0, 0));
-      }
+        for (int p = 0; p < KD; ++p)
+          f[e * KD + p] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(b.v[0], vo[p] + e * rb, 0, 0));
     }
   }
 
-  __device__ __forceinline__ static bool nonfinite(const Block& b) {
+  __device__ __forceinline__ static bool nonfinite(const uint4 (&v)[NV]) {
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t w[4] = {b.v[i].x, b.v[i].y, b.v[i].z, b.v[i].w};
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         bad |= (w[j] & 0x7f800000u) == 0x7f800000u;
@@ -251,8 +277,8 @@ struct Walk {
 
   // P.V of a partly masked block whose values are not all finite, key by key: a key adds nothing (not even
   // 0 x infinity) to the rows that do not see it. Rare: reads the values again.
-  __device__ __forceinline__ void masked_pv(const Block& b, const float (&p)[4 * KT], f32x4 (&o)[DT], int k0, int lo,
-                                            int hi) {
+  __device__ __forceinline__ void masked_pv(const Tiles& b, const float (&p)[4 * KT], f32x4 (&o)[DT], int k0, int lo,
+                                            int hi) const {
 #pragma nounroll
     for (int i = 0; i < 4 * KT; ++i) {
       float pi = p[0];
@@ -276,127 +302,15 @@ struct Walk {
     }
   }
 
-  // Scores, online softmax and P.V of one block. Row (column c of tile t) sees keys [lo[t], hi[t]). full: every row
-  // sees the whole block.
-  __device__ __forceinline__ void step(const Block& b, int k0, const int (&lo)[NT], const int (&hi)[NT], bool full) {
-    bool slow = false;
-    if (!full) slow = __any(nonfinite(b));
-    if constexpr (kBf16) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int row = i * (64 / LPR) + lane / LPR, d = (lane % LPR) * 8;
-        if (KD != 3 || d < 32 * KD) *reinterpret_cast<uint4*>(vt + row * LD + d) = b.v[i];
-      }
-    }
-    float p[NT][4 * KT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      f32x4 s[KT];
-#pragma unroll
-      for (int u = 0; u < KT; ++u) {
-        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (kBf16) {
-#pragma unroll
-          for (int k = 0; k < KD; ++k)
-            s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.k[u * KD + k]),
-                                                           __builtin_bit_cast(bf16x8, qf[t][k]), s[u], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 2 * KD; ++k) {
-            const f32x4 kf = __builtin_bit_cast(f32x4, b.k[k]), q4 = __builtin_bit_cast(f32x4, qf[t][k]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], q4[e], s[u], 0, 0, 0);
-          }
-        }
-      }
-      uint32_t vis = 0xffffffffu;
-      float mx = -INFINITY;
-      if (!full) {
-        vis = 0;
-#pragma unroll
-        for (int u = 0; u < KT; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = k0 + 16 * u + 4 * g + r;
-            if (key >= lo[t] && key < hi[t] && b.ok[u]) vis |= 1u << (4 * u + r);
-          }
-      }
-#pragma unroll
-      for (int i = 0; i < 4 * KT; ++i) {
-        const float x = s[i >> 2][i & 3];
-        mx = fmaxf(mx, (full || (vis >> i & 1)) ? x : -INFINITY);
-      }
-      const float mn = fmaxf(m[t], xmax(mx));
-      const float mc = mn == -INFINITY ? 0.f : mn * kLog2e;
-      if (__any(mn != m[t])) {
-        const float f = __builtin_amdgcn_exp2f(fmaf(m[t], kLog2e, -mc));
-        l[t] *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[t][d] *= f;
-        m[t] = mn;
-      }
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4 * KT; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], kLog2e, -mc));
-        p[t][i] = (full || (vis >> i & 1)) ? e : 0.f;
-        sum += p[t][i];
-      }
-      l[t] += sum;
-    }
-    if (slow) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) masked_pv(b, p[t], acc[t], k0, lo[t], hi[t]);
-      return;
-    }
-    if constexpr (kBf16) {
-      // P in bf16 for the matrix product (as esgpt_attn_fwd and esgpt_attn_decode round it; the sums stay f32)
-      bf16x8 pf[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pf[t][i] = (__bf16)p[t][i];
-      const __bf16* vr = vt + (4 * g + (c >> 2)) * LD + 4 * (c & 3);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        typedef __attribute__((address_space(3))) bf16x4* lds4;
-        const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * d));
-        const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * LD + 16 * d));
-        bf16x8 vf;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          vf[i] = x[i];
-          vf[4 + i] = y[i];
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], acc[t][d], 0, 0, 0);
-      }
-    } else {
-      const float* v = reinterpret_cast<const float*>(b.v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[(e * KD + (d >> 1)) * 2 + (d & 1)], p[t][e], acc[t][d],
-                                                             0, 0, 0);
-    }
-  }
-
-  // Page ids of the next 64 / KT blocks of this wave, one lane each; -1: past the end or not a page.
-  __device__ __forceinline__ int pages(const int32_t* tab, int k0, int stride, int k_end) {
-    const int key = k0 + (lane / KT) * stride + (lane % KT) * 16;
-    if (key >= k_end) return -1;
-    const int id = tab[key >> a.psl];
-    if (id >= 0 && id < a.n_pages) return id;
-    set_err(a.err, ESGPT_FLAG_BAD_PAGE);
-    return -1;
-  }
-
-  // Blocks k_first, k_first + stride, ... below k_end of the rows named by tab. k_first is a multiple of 16.
-  __device__ __forceinline__ void walk(const int32_t* tab, int k_first, int stride, int k_end, const int (&lo)[NT],
-                                       const int (&hi)[NT], const bool (&act)[NT]) {
+  // Blocks k_first, k_first + stride, ... below k_end of the rows that tab names; raw: pages() of the first ones.
+  // Row (column c of tile t) sees keys [lo[t], hi[t]). k_first is a multiple of 16. A block's V goes to LDS at the top
+  // of its step and its K to the matrix units right after, and the next block's loads follow each: one set of
+  // registers, a whole step of latency covered.
+  template <int NT>
+  __device__ __forceinline__ void walk(State<NT, DT>& st, const Q (&qf)[NT], const int32_t* tab, int raw, int k_first,
+                                       int stride, int k_end, const int (&lo)[NT], const int (&hi)[NT],
+                                       const bool (&act)[NT]) const {
+    if (k_first >= k_end) return;
     int lo_all = 0, hi_all = 0x7fffffff;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -404,27 +318,129 @@ struct Walk {
         lo_all = max(lo_all, lo[t]);
         hi_all = min(hi_all, hi[t]);
       }
+    int pid = check(raw, k_first, stride, k_end), slot = 0;
+    Tiles b = tiles(k_first, k_end, pid, 0);
+    uint4 k[KT * NK], v[NV];
+    load_k(k, b);
+    load_v(v, b);
     lo_all = wave_max_i(lo_all);
     hi_all = wave_min_i(hi_all);
-    if (k_first >= k_end) return;
-    constexpr int PER = 64 / KT;
-    int pid = pages(tab, k_first, stride, k_end), slot = 0;
-    Block b, nx;
-    load(b, k_first, k_end, pid, 0);
-    for (int k0 = k_first; k0 < k_end; k0 += stride) {
+    for (int k0 = k_first;; k0 += stride) {
       const int k1 = k0 + stride;
-      if (k1 < k_end) {
+      const bool more = k1 < k_end;
+      Tiles nb = b;
+      if (more) {
         if (++slot == PER) {
           slot = 0;
-          pid = pages(tab, k1, stride, k_end);
+          pid = check(pages(tab, k1, stride, k_end), k1, stride, k_end);
         }
-        load(nx, k1, k_end, pid, slot);
+        nb = tiles(k1, k_end, pid, slot);
       }
       bool full = k0 >= lo_all && k0 + KB <= hi_all && k0 + KB <= k_end;
 #pragma unroll
       for (int t = 0; t < KT; ++t) full = full && b.ok[t];
-      step(b, k0, lo, hi, full);
-      if (k1 < k_end) b = nx;
+      bool slow = false;
+      if (!full) slow = __any(nonfinite(v));
+      if constexpr (kBf16) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int row = i * (64 / LPR) + lane / LPR, d = (lane % LPR) * 8;
+          if (KD != 3 || d < 32 * KD) *reinterpret_cast<uint4*>(vt + row * LD + d) = v[i];
+        }
+        if (more) load_v(v, nb);
+      }
+      f32x4 s[NT][KT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+          s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if constexpr (kBf16) {
+#pragma unroll
+            for (int i = 0; i < KD; ++i)
+              s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u * KD + i]),
+                                                                __builtin_bit_cast(bf16x8, qf[t][i]), s[t][u], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2 * KD; ++i) {
+              const f32x4 kf = __builtin_bit_cast(f32x4, k[i]), q4 = __builtin_bit_cast(f32x4, qf[t][i]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], q4[e], s[t][u], 0, 0, 0);
+            }
+          }
+        }
+      if (more) load_k(k, nb);
+      float p[NT][4 * KT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (!full) {
+#pragma unroll
+          for (int i = 0; i < 4 * KT; ++i) {
+            const int key = k0 + 16 * (i >> 2) + 4 * g + (i & 3);
+            // a masked score is -inf (it may be NaN); its probability is then an exact zero
+            if (!(key >= lo[t] && key < hi[t] && b.ok[i >> 2])) s[t][i >> 2][i & 3] = -INFINITY;
+          }
+        }
+        float mx = s[t][0][0];
+#pragma unroll
+        for (int i = 1; i < 4 * KT; ++i) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
+        const float mn = fmaxf(st.m[t], xmax(mx));
+        const float mc = mn == -INFINITY ? 0.f : mn * kLog2e;
+        if (__any(mn != st.m[t])) {
+          const float f = __builtin_amdgcn_exp2f(fmaf(st.m[t], kLog2e, -mc));
+          st.l[t] *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) st.acc[t][d] *= f;
+          st.m[t] = mn;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * KT; ++i) {
+          p[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], kLog2e, -mc));
+          sum += p[t][i];
+        }
+        st.l[t] += sum;
+      }
+      if (slow) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) masked_pv(b, p[t], st.acc[t], k0, lo[t], hi[t]);
+      } else if constexpr (kBf16) {
+        // P in bf16 for the matrix product (as esgpt_attn_fwd and esgpt_attn_decode round it; the sums stay f32)
+        bf16x8 pf[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pf[t][i] = (__bf16)p[t][i];
+        const __bf16* vr = vt + (4 * g + (c >> 2)) * LD + 4 * (c & 3);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          typedef __attribute__((address_space(3))) bf16x4* lds4;
+          const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * d));
+          const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * LD + 16 * d));
+          bf16x8 vf;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            vf[i] = x[i];
+            vf[4 + i] = y[i];
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], st.acc[t][d], 0, 0, 0);
+        }
+      } else {
+        const float* f = reinterpret_cast<const float*>(v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[(e * KD + (d >> 1)) * 2 + (d & 1)], p[t][e],
+                                                                  st.acc[t][d], 0, 0, 0);
+      }
+      if (!more) break;
+      if constexpr (!kBf16) load_v(v, nb);
+      b = nb;
     }
   }
 };
@@ -456,129 +472,202 @@ __device__ __forceinline__ void emit4(const SharedArgs& a, int64_t out, int h, i
   if (l != 0.f) *reinterpret_cast<float4*>(a.po + at * a.hd + d) = v;  // l == 0: the join does not read it
 }
 
-// The four waves' states of column tile t, joined per row through LDS: row r0 + i of the group (i < 16).
-template <typename T, int KD, int t, typename W>
-__device__ __forceinline__ void join_waves(const SharedArgs& a, const W& x, bool act, char* lds, int64_t out0, int r0,
-                                           int h, int ch) {
-  constexpr int OLD = KD * 32 + 4;
-  const int w = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, c = lane & 15;
-  float* jo = reinterpret_cast<float*>(lds);  // [wave][16][OLD]
-  float* jm = jo + kWaves * 16 * OLD;         // [wave][16]
-  float* jl = jm + kWaves * 16;
-  __syncthreads();  // the waves' V tiles, or the tile before
-  const float lw = act ? xsum(x.l[t]) : 0.f;
-  if (g == 0) {
-    jm[w * 16 + c] = x.m[t];
-    jl[w * 16 + c] = lw;
-  }
+// The waves' states of one tile of 16 rows, joined per row through LDS, 64 dimensions at a time: row r0 + i of the group
+// is column i. Every thread of the workgroup calls this.
+template <typename T, int KD, int NW>
+struct Join {
+  static constexpr int W = KD * 32 < 64 ? KD * 32 : 64, OLD = W + 4;
+  static constexpr int kBytes = NW * 16 * (OLD + 2) * 4;
+  template <int NT>
+  __device__ __forceinline__ static void run(const SharedArgs& a, const State<NT, 2 * KD>& st, int t, bool act, char* lds,
+                                             int64_t out0, int r0, int h, int part) {
+    const int w = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, c = lane & 15;
+    float* jo = reinterpret_cast<float*>(lds);  // [wave][16][OLD]
+    float* jm = jo + NW * 16 * OLD;             // [wave][16]
+    float* jl = jm + NW * 16;
+    const float lw = act ? xsum(st.l[t]) : 0.f;
+    const int row = threadIdx.x >> 4;
+    const bool mine = row < 16 && r0 + row < a.M;
+    float M = -INFINITY, L = 0.f;
 #pragma unroll
-  for (int d = 0; d < W::DT; ++d) {
-    int dim;
-    const float4 v = four<T, W::DT>(x.acc[t], d, g, dim);
-    *reinterpret_cast<float4*>(jo + (w * 16 + c) * OLD + dim) = v;
-  }
-  __syncthreads();
-  const int row = threadIdx.x >> 4;
-  if (r0 + row >= a.M) return;
-  float M = -INFINITY, L = 0.f, f[kWaves];
+    for (int d0 = 0; d0 < KD * 32; d0 += W) {
+      __syncthreads();  // the waves' V tiles, or the reads of the round before
+      if (d0 == 0 && g == 0) {
+        jm[w * 16 + c] = st.m[t];
+        jl[w * 16 + c] = lw;
+      }
 #pragma unroll
-  for (int u = 0; u < kWaves; ++u) M = fmaxf(M, jl[u * 16 + row] == 0.f ? -INFINITY : jm[u * 16 + row]);
-  const float mc = M == -INFINITY ? 0.f : M * kLog2e;
-#pragma unroll
-  for (int u = 0; u < kWaves; ++u) {
-    const float lu = jl[u * 16 + row];
-    f[u] = __builtin_amdgcn_exp2f(fmaf(jm[u * 16 + row], kLog2e, -mc));
-    if (lu != 0.f) L = fmaf(lu, f[u], L);
-  }
-  for (int d = 4 * (threadIdx.x & 15); d < a.hd; d += 64) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < kWaves; ++u) {
-      if (jl[u * 16 + row] == 0.f) continue;  // this wave saw nothing for the row
-      const float4 y = *reinterpret_cast<const float4*>(jo + (u * 16 + row) * OLD + d);
-      v.x = fmaf(y.x, f[u], v.x);
-      v.y = fmaf(y.y, f[u], v.y);
-      v.z = fmaf(y.z, f[u], v.z);
-      v.w = fmaf(y.w, f[u], v.w);
+      for (int d = 0; d < 2 * KD; ++d) {
+        int dim;
+        const float4 v = four<T, 2 * KD>(st.acc[t], d, g, dim);
+        if (d / (W / 16) == d0 / W) *reinterpret_cast<float4*>(jo + (w * 16 + c) * OLD + dim - d0) = v;
+      }
+      __syncthreads();
+      if (!mine) continue;
+      if (d0 == 0) {
+        for (int u = 0; u < NW; ++u) M = fmaxf(M, jl[u * 16 + row] == 0.f ? -INFINITY : jm[u * 16 + row]);
+      }
+      const float mc = M == -INFINITY ? 0.f : M * kLog2e;
+      const int d = d0 + 4 * (threadIdx.x & 15);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float Ls = 0.f;
+      for (int u = 0; u < NW; ++u) {
+        const float lu = jl[u * 16 + row];
+        if (lu == 0.f) continue;  // this wave saw nothing for the row
+        const float f = __builtin_amdgcn_exp2f(fmaf(jm[u * 16 + row], kLog2e, -mc));
+        Ls = fmaf(lu, f, Ls);
+        if (d - d0 >= W) continue;
+        const float4 y = *reinterpret_cast<const float4*>(jo + (u * 16 + row) * OLD + d - d0);
+        v.x = fmaf(y.x, f, v.x);
+        v.y = fmaf(y.y, f, v.y);
+        v.z = fmaf(y.z, f, v.z);
+        v.w = fmaf(y.w, f, v.w);
+      }
+      if (d0 == 0) L = Ls;
+      if (d - d0 < W && d < a.hd) emit4<T>(a, out0 + r0 + row, h, part, d, v, M, L, d == 0);
     }
-    emit4<T>(a, out0 + r0 + row, h, ch, d, v, M, L, d == 0);
   }
-}
+};
 
+// Split form: a workgroup per history chunk of one (group, head, 16 NT rows), then four waves a workgroup with the own
+// rows of one (trajectory, head, chunk) each.
 template <typename T, int KD, int NT>
 __global__ __launch_bounds__(64 * kWaves) void shared_kernel(SharedArgs a) {
-  using W = Walk<T, KD, NT>;
-  constexpr int OLD = KD * 32 + 4;
+  using W = Walk<T, KD>;
+  using J = Join<T, KD, kWaves>;
   constexpr int kTile = W::kBf16 ? W::KB * W::LD * 2 : 0;
-  constexpr int kJoin = kWaves * 16 * (OLD + 2) * 4;
-  __shared__ __align__(16) char lds[(kWaves * kTile > kJoin) ? kWaves * kTile : kJoin];
+  __shared__ __align__(16) char lds[(kWaves * kTile > J::kBytes) ? kWaves * kTile : J::kBytes];
   const int w = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, c = lane & 15;
 
   if ((int)blockIdx.x >= a.units) {
-    // own rows of one (trajectory, head, chunk) per wave: column c is its new event c
-    const int64_t id = (int64_t)(blockIdx.x - a.units) * kWaves + w;
-    const int ch = (int)(id % a.NSc), h = (int)(id / a.NSc % a.H), s = (int)(id / a.NSc / a.H);
+    // column c is the trajectory's new event c
+    const int id = (int)(blockIdx.x - a.units) * kWaves + w;
+    const int ch = id % a.NSc, sh = id / a.NSc, h = sh % a.H, s = sh / a.H;
     if (s >= a.S) return;
-    using W1 = Walk<T, KD, 1>;
-    W1 x(a, h, lds + w * kTile);
+    const W x(a, h, lds + w * kTile);
+    const int32_t* tab = a.table + (int64_t)s * a.table_w;
+    int raw = a.window ? -1 : x.pages(tab, ch * a.schunk, W::KB, a.cap);
     const Row r = row_of(a, s, c, c < a.Lq);
-    x.load_q(0, r);
+    typename W::Q q[1];
+    x.load_q(q[0], r);
     const int hi = r.active ? min(r.at + 1, a.cap) : 0, lo = (r.active && a.window) ? max(0, r.at - a.window + 1) : 0;
-    const int base = wave_min_i(r.active ? lo : 0x7fffffff) & ~15;  // no active row: no key
-    const int end = wave_max_i(hi);
-    const int64_t first = (int64_t)base + (int64_t)ch * a.schunk;
+    const int base = wave_min_i(r.active ? lo : a.cap) & ~15;  // no active row: no key
+    const int end = wave_max_i(hi), first = base + ch * a.schunk;
+    if (a.window && first < end) raw = x.pages(tab, first, W::KB, end);
+    State<1, W::DT> st;
+    st.clear();
     const int los[1] = {lo}, his[1] = {hi};
     const bool act[1] = {r.active};
-    if (first < end)
-      x.walk(a.table + (int64_t)s * a.table_w, (int)first, W1::KB, (int)min((int64_t)end, first + a.schunk), los, his, act);
-    const float l = r.active ? xsum(x.l[0]) : 0.f;
+    x.walk(st, q, tab, raw, first, W::KB, min(end, first + a.schunk), los, his, act);
+    const float l = r.active ? xsum(st.l[0]) : 0.f;
     if (c < a.Lq) {
-      const int64_t out = (int64_t)s * a.Lq + c;
 #pragma unroll
-      for (int d = 0; d < W1::DT; ++d) {
+      for (int d = 0; d < W::DT; ++d) {
         int dim;
-        const float4 v = four<T, W1::DT>(x.acc[0], d, g, dim);
-        if (dim < a.hd) emit4<T>(a, out, h, a.NPc + ch, dim, v, x.m[0], l, d == 0 && g == 0);
+        const float4 v = four<T, W::DT>(st.acc[0], d, g, dim);
+        if (dim < a.hd) emit4<T>(a, (int64_t)s * a.Lq + c, h, a.NPc + ch, dim, v, st.m[0], l, d == 0 && g == 0);
       }
     }
     return;
   }
 
-  // history chunk of one (group, head, 16 NT rows): neighbouring workgroups of one XCD share a chunk's keys and values
+  // neighbouring workgroups of one XCD share a chunk's keys and values
   const int id = xcd_linear(blockIdx.x, a.units);
   const int rt = id % a.RT, ch = id / a.RT % a.NPc, gh = id / a.RT / a.NPc;
   const int h = gh % a.H, grp = gh / a.H;
-  W x(a, h, lds + w * kTile);
+  const W x(a, h, lds + w * kTile);
+  const int32_t* tab = a.prefix_table + (int64_t)grp * a.prefix_w;
+  constexpr int kStride = kWaves * W::KB;
+  int raw = a.window ? -1 : x.pages(tab, ch * a.pchunk + w * W::KB, kStride, a.prefix_cap);
   const int P = prefix_len(a, grp);
-  int lo[NT], hi[NT], base = 0x7fffffff;
+  int lo[NT], hi[NT], base = a.prefix_cap;
   bool act[NT];
-  Row rows[NT];
+  typename W::Q q[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int rr = rt * 16 * NT + 16 * t + c;
-    rows[t] = row_of(a, grp * a.n + rr / a.Lq, rr % a.Lq, rr < a.M);
-    x.load_q(t, rows[t]);
-    act[t] = rows[t].active;
+    const Row r = row_of(a, grp * a.n + rr / a.Lq, rr % a.Lq, rr < a.M);
+    x.load_q(q[t], r);
+    act[t] = r.active;
     hi[t] = act[t] ? P : 0;
-    lo[t] = (act[t] && a.window) ? min(P, max(0, P + rows[t].at - a.window + 1)) : 0;
+    lo[t] = (act[t] && a.window) ? min(P, max(0, P + r.at - a.window + 1)) : 0;
     if (act[t]) base = min(base, lo[t]);
   }
   // chunks count from the first row that a window of this group can reach, whatever its own rows
-  const int from = (a.window ? max(0, P - a.window) : 0) & ~15;
-  const int64_t c0 = (int64_t)from + (int64_t)ch * a.pchunk;
-  const int64_t end = min((int64_t)P, c0 + a.pchunk);
-  base = wave_min_i(base) & ~15;
-  int64_t first = c0 + (int64_t)w * W::KB;
-  if (base > c0) {  // whole rounds of blocks before the first visible key
-    const int64_t skip = (base - c0) / (kWaves * W::KB) * (kWaves * W::KB);
-    first += skip;
+  const int c0 = ((a.window ? max(0, P - a.window) : 0) & ~15) + ch * a.pchunk, end = min(P, c0 + a.pchunk);
+  int first = c0 + w * W::KB;
+  if (a.window) {  // whole rounds of blocks before the first visible key
+    first += max(0, (wave_min_i(base) & ~15) - c0) / kStride * kStride;
+    if (first < end) raw = x.pages(tab, first, kStride, end);
   }
-  if (first < end)
-    x.walk(a.prefix_table + (int64_t)grp * a.prefix_w, (int)first, kWaves * W::KB, (int)end, lo, hi, act);
-
+  State<NT, W::DT> st;
+  st.clear();
+  x.walk(st, q, tab, raw, first, kStride, end, lo, hi, act);
   const int64_t out0 = (int64_t)grp * a.M;
-  join_waves<T, KD, 0>(a, x, act[0], lds, out0, rt * 16 * NT, h, ch);
-  if constexpr (NT == 2) join_waves<T, KD, 1>(a, x, act[1], lds, out0, rt * 16 * NT + 16, h, ch);
+  J::run(a, st, 0, act[0], lds, out0, rt * 16 * NT, h, ch);
+  if constexpr (NT == 2) J::run(a, st, 1, act[1], lds, out0, rt * 16 * NT + 16, h, ch);
+}
+
+// Whole form: one workgroup of NW waves per (group, head, 16 rows) does the rows' history and their own rows and writes
+// the result. The waves take every NW-th block of the history and, from the other end, every NW-th trajectory.
+template <typename T, int KD, int NW>
+__global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
+  using W = Walk<T, KD>;
+  using J = Join<T, KD, NW>;
+  constexpr int kTile = W::kBf16 ? W::KB * W::LD * 2 : 0;
+  __shared__ __align__(16) char lds[(NW * kTile > J::kBytes) ? NW * kTile : J::kBytes];
+  const int w = threadIdx.x >> 6, lane = lane_id(), c = lane & 15;
+  const int id = xcd_linear(blockIdx.x, gridDim.x);
+  const int rt = id % a.RT, gh = id / a.RT, h = gh % a.H, grp = gh / a.H;
+  const W x(a, h, lds + w * kTile);
+  const int32_t* ptab = a.prefix_table + (int64_t)grp * a.prefix_w;
+  constexpr int kStride = NW * W::KB;
+  const int rr = rt * 16 + c;
+  const int s0 = grp * a.n + rt * 16 / a.Lq, ns = grp * a.n + min(a.M - 1, rt * 16 + 15) / a.Lq - s0 + 1;
+  const int ow = NW - 1 - w;
+  // page ids that need no length: of the history, and of this wave's first trajectory
+  int raw = a.window ? -1 : x.pages(ptab, w * W::KB, kStride, a.prefix_cap);
+  int oraw = a.window || ow >= ns ? -1 : x.pages(a.table + (int64_t)(s0 + ow) * a.table_w, 0, W::KB, a.cap);
+  const int P = prefix_len(a, grp);
+  const int my = grp * a.n + rr / a.Lq;  // this column's trajectory
+  const Row r = row_of(a, my, rr % a.Lq, rr < a.M);
+  typename W::Q q[1];
+  x.load_q(q[0], r);
+  State<1, W::DT> st;
+  st.clear();
+  {
+    const int lo[1] = {(r.active && a.window) ? min(P, max(0, P + r.at - a.window + 1)) : 0}, hi[1] = {r.active ? P : 0};
+    const bool act[1] = {r.active};
+    int first = w * W::KB;
+    if (a.window) {
+      first += wave_min_i(r.active ? lo[0] : P) & ~15;
+      if (first < P) raw = x.pages(ptab, first, kStride, P);
+    }
+    x.walk(st, q, ptab, raw, first, kStride, P, lo, hi, act);
+  }
+  for (int j = ow; j < ns; j += NW) {
+    const int s = s0 + j;
+    const int32_t* tab = a.table + (int64_t)s * a.table_w;
+    const bool act[1] = {r.active && my == s};
+    const int lo[1] = {(act[0] && a.window) ? max(0, r.at - a.window + 1) : 0}, hi[1] = {act[0] ? min(r.at + 1, a.cap) : 0};
+    const int first = wave_min_i(act[0] ? lo[0] : a.cap) & ~15, end = wave_max_i(hi[0]);
+    if (first >= end) continue;
+    if (a.window || j != ow) oraw = x.pages(tab, first, W::KB, end);
+    State<1, W::DT> own;
+    own.clear();
+    x.walk(own, q, tab, oraw, first, W::KB, end, lo, hi, act);
+    // into this wave's state, the trajectory's columns only
+    const float mn = fmaxf(st.m[0], own.m[0]), mc = mn == -INFINITY ? 0.f : mn * kLog2e;
+    const float fa = __builtin_amdgcn_exp2f(fmaf(st.m[0], kLog2e, -mc));
+    const float fb = __builtin_amdgcn_exp2f(fmaf(own.m[0], kLog2e, -mc));
+    if (act[0]) {
+      st.m[0] = mn;
+      st.l[0] = fmaf(st.l[0], fa, own.l[0] * fb);
+#pragma unroll
+      for (int d = 0; d < W::DT; ++d) st.acc[0][d] = st.acc[0][d] * fa + own.acc[0][d] * fb;
+    }
+  }
+  J::run(a, st, 0, r.active, lds, (int64_t)grp * a.M, rt * 16, h, 0);
 }
 
 // Joins a row's parts: o = sum_p e^{m_p - M} O_p / sum_p e^{m_p - M} l_p. One wave per (row, head): lane groups of
@@ -618,23 +707,41 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a, int64_t 
 }
 
 struct SharedPlan {
-  int NT, RT, NPc, NSc, NP, pchunk, schunk;
+  int whole, NT, RT, NPc, NSc, NP, pchunk, schunk;
   int64_t units, own_blocks;
 };
 
-SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t prefix_cap, int64_t cap, int64_t window,
-                       int dtype) {
+// Waves of the whole form's workgroup: past 64 dimensions a wave's registers and LDS leave room for four.
+int whole_waves(int64_t hd) { return hd <= 64 ? 8 : 4; }
+constexpr int64_t kWholeSteps = 8, kWholeUnits = 1024;
+
+SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap, int64_t cap,
+                       int64_t window, int dtype) {
   SharedPlan p;
   const int64_t M = (S / G) * Lq, kb = dtype == ESGPT_BF16 ? 32 : 16;
+  const int64_t pspan = window ? std::min(prefix_cap, window + 16) : prefix_cap;
+  const int64_t sspan = window ? std::min(cap, window + Lq + 16) : cap;
+  {
+    // whole form: blocks of keys that its busiest wave walks one after the other
+    const int64_t seqs = std::min<int64_t>(cdiv(std::min<int64_t>(M, 16), Lq) + (Lq > 1), S / G);
+    const int64_t nw = whole_waves(hd), steps = cdiv(pspan, nw * kb) + cdiv(seqs, nw) * cdiv(sspan, kb);
+    p.RT = (int)cdiv(M, 16);
+    p.units = G * H * p.RT;
+    p.whole = steps <= kWholeSteps || p.units >= kWholeUnits;
+    if (p.whole) {
+      p.NT = p.NP = 1;
+      p.NPc = p.NSc = p.pchunk = p.schunk = 0;
+      p.own_blocks = 0;
+      return p;
+    }
+  }
   p.NT = dtype == ESGPT_BF16 && M > 16 ? 2 : 1;
   p.RT = (int)cdiv(M, 16 * p.NT);
   const int64_t round = kWaves * kb;
-  const int64_t pspan = window ? std::min(prefix_cap, window + 16) : prefix_cap;
   const int64_t base = G * H * p.RT;
   p.NPc = pspan ? (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, base), cdiv(pspan, round), 48})) : 0;
   p.pchunk = p.NPc ? (int)(cdiv(cdiv(pspan, p.NPc), round) * round) : 0;
   p.NPc = p.NPc ? (int)cdiv(pspan, p.pchunk) : 0;
-  const int64_t sspan = window ? std::min(cap, window + Lq + 16) : cap;
   p.NSc = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(4096, S * H), cdiv(sspan, 2 * kb), 16}));
   p.schunk = (int)(cdiv(cdiv(sspan, p.NSc), kb) * kb);
   p.NSc = (int)cdiv(sspan, p.schunk);
@@ -648,6 +755,15 @@ template <typename T>
 int launch_shared(const SharedPlan& p, const SharedArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(p.units + p.own_blocks)), block(64 * kWaves);
   const int kd = (a.hd + 31) / 32;
+  if (p.whole) {
+    const dim3 wide(64 * whole_waves(a.hd));
+    if (kd == 1) shared_whole_kernel<T, 1, 8><<<grid, wide, 0, st>>>(a);
+    else if (kd == 2) shared_whole_kernel<T, 2, 8><<<grid, wide, 0, st>>>(a);
+    else if (kd == 3) shared_whole_kernel<T, 3, 4><<<grid, wide, 0, st>>>(a);
+    else shared_whole_kernel<T, 4, 4><<<grid, wide, 0, st>>>(a);
+    ESGPT_LAUNCH_CHECK();
+    return ESGPT_OK;
+  }
 #define SHARED(KD)                                                                        \
   do {                                                                                    \
     if constexpr (sizeof(T) == 2) {                                                       \
@@ -689,7 +805,7 @@ extern "C" {
 size_t esgpt_attn_decode_shared_workspace(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap,
                                           int64_t cap, int64_t window, int dtype) {
   if (!shared_ok(G, S, Lq, H, hd, prefix_cap, cap, window, dtype)) return 0;
-  const SharedPlan p = shared_plan(G, S, Lq, H, prefix_cap, cap, std::min<int64_t>(window, (int64_t)1 << 30), dtype);
+  const SharedPlan p = shared_plan(G, S, Lq, H, hd, prefix_cap, cap, std::min<int64_t>(window, (int64_t)1 << 30), dtype);
   return p.NP > 1 ? (size_t)(S * Lq * H * p.NP) * (2 + hd) * sizeof(float) : 0;
 }
 
@@ -707,7 +823,7 @@ int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_p
   ESGPT_REQUIRE(q && o && past && page_table && aligned(q) && aligned(o) && (prefix_cap == 0 || (prefix_table && prefix_lens)));
   ESGPT_REQUIRE(n_pages == 0 || (k_pages && v_pages && aligned(k_pages) && aligned(v_pages)));
   window = std::min<int64_t>(window, (int64_t)1 << 30);
-  const SharedPlan p = shared_plan(G, S, Lq, H, prefix_cap, cap, window, dtype);
+  const SharedPlan p = shared_plan(G, S, Lq, H, hd, prefix_cap, cap, window, dtype);
   ESGPT_REQUIRE(p.units + p.own_blocks < (int64_t)1 << 31);
   SharedArgs a{};
   if (p.NP > 1) {

@@ -412,6 +412,8 @@ def _lib():
 
     if not os.path.exists(L.LIB_PATH):
         pytest.skip("library not built")
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses: only where no device could read them")
     return L.load(require_device=False)
 
 
