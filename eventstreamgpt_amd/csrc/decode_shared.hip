@@ -13,14 +13,21 @@
 // nothing as long as memory is the bound (a bf16 tile of 16 keys x 64 takes 64 MFMA cycles for 4 KB, 64 B per cycle and
 // SIMD, against the 13 B per cycle that HBM gives a whole CU).
 //
-// Split: the history of each (group, head, 16 or 32 rows) is cut into chunks (one workgroup each, its four waves taking
-// every fourth 32-key block and joining through LDS), the own rows of each (trajectory, head) into chunks of one wave.
-// Each part leaves (m, l, O) in f32 and a second kernel joins a row's parts; with one part in all the result is
-// written directly. The cut follows the caller's bounds on the lengths (the lengths themselves are on the device).
+// Two forms (shared_plan chooses and holds the measurements). Whole: one workgroup per (group, head, 16 rows) does the
+// history and the own rows and writes the result. Split: the history of each (group, head, 16 or 32 rows) is cut into
+// chunks, one workgroup each, whose four waves take every fourth block of keys and join through LDS, and the own rows of
+// each (trajectory, head) into chunks of one wave; each part leaves (m, l, O) in f32 and a second kernel joins a row's
+// parts. The cut follows the caller's bounds on the lengths (the lengths themselves are on the device).
+//
+// A wave keeps 16 KB of keys and values in flight (Walk::pass). What it walks by is scalar: page places, ends, buffer
+// descriptors. Measured with those in vector registers (a wave's number taken from threadIdx, a length loaded like data),
+// every buffer load became a loop over the lanes: 3,555 vector instructions a wave against 1,622, 32 x 16 over 256 + 64
+// events 15.5 us against 13.1; 64 keys a block rather than 32, 8 x 32 over 16,384 events 59.5 -> 58.9 at 512 chunks.
+// Now 8 x 32 over 16,384 + 64 (hd 64, 8 heads, bf16) takes 52 us + 4 of join: 5.0 TB/s, what a large copy reaches.
 //
 // Nothing is read beyond a sequence's length: rows past it are zeros in registers, so what an unused part of a page
 // holds (NaN, infinity) never meets a product. Where a tile is partly masked (a window's edge, a later event of the same
-// call), 0 x infinity is kept out of the other rows by an exact path (masked_pv).
+// call), 0 x infinity is kept out of the other rows by an exact second pass (masked_pv).
 #include "common.h"
 
 #include <algorithm>
@@ -65,30 +72,37 @@ __device__ __forceinline__ float xsum(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-__device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return __builtin_amdgcn_readfirstlane(v);
+// A value that is the same in every lane, in a scalar register: buffer descriptors, page places and loop bounds that the
+// compiler finds in vector registers cost a loop over the lanes at each use.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Smallest / largest value over the sixteen columns (a column's four lanes hold the same), as a scalar.
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false); }
+__device__ __forceinline__ int cols_min(int v) {
+  v = min(v, dpp_i<0xB1>(v));
+  v = min(v, dpp_i<0x4E>(v));
+  v = min(v, dpp_i<0x141>(v));
+  v = min(v, dpp_i<0x140>(v));
+  return scalar(v);
 }
-__device__ __forceinline__ int wave_max_i(int v) { return -wave_min_i(-v); }
+__device__ __forceinline__ int cols_max(int v) { return -cols_min(-v); }
 
 // One new event: its place among its trajectory's own rows. active: it exists, is not padding and its past is sane.
 struct Row {
-  int64_t out;  // row of q and o
-  int at;       // own row
+  int at;  // own row
   bool active;
 };
 __device__ __forceinline__ Row row_of(const SharedArgs& a, int s, int i, bool exists) {
-  Row r{0, 0, false};
+  Row r{0, false};
   if (!exists) return r;
-  r.out = (int64_t)s * a.Lq + i;
   const int past = a.past[s];
   int k = i;
   bool keep = true;
   if (a.row_mask) {
     k = 0;
     for (int j = 0; j < i; ++j) k += a.row_mask[(int64_t)s * a.Lq + j] != 0;
-    keep = a.row_mask[r.out] != 0;
+    keep = a.row_mask[(int64_t)s * a.Lq + i] != 0;
   }
   if (!keep) return r;
   if (past < 0 || past > a.cap - 1 - k) {  // a row that the cache has no place for
@@ -103,7 +117,7 @@ __device__ __forceinline__ int prefix_len(const SharedArgs& a, int g) {
   if (a.prefix_cap == 0) return 0;
   const int P = a.prefix_lens[g];
   if (P < 0 || P > a.prefix_cap) set_err(a.err, ESGPT_FLAG_BAD_PAGE);
-  return min(max(P, 0), a.prefix_cap);
+  return scalar(min(max(P, 0), a.prefix_cap));
 }
 
 // Dimension of accumulator register r of tile dt in lane group g (= lane / 16). bf16: the transposed V tile's natural
@@ -148,13 +162,15 @@ struct State {
 template <typename T, int KD>
 struct Walk {
   static constexpr bool kBf16 = sizeof(T) == 2;
-  static constexpr int KT = kBf16 ? 2 : 1;  // 16-key tiles per block: both types move 8 KB (hd 64) per block and wave
+  // 16-key tiles per block: 16 KB of keys and values per block and wave at 64 dimensions and at 128 in bf16
+  static constexpr int KT = kBf16 ? (KD <= 2 ? 4 : 2) : (KD <= 2 ? 2 : 1);
   static constexpr int KB = 16 * KT;
   static constexpr int DT = 2 * KD;        // 16-wide tiles of the head
   static constexpr int LD = KD * 32 + 16;  // LDS row of V (elements): 8 mod 16 dwords, transposed reads hit all banks
   static constexpr int NK = kBf16 ? KD : 2 * KD;     // 16-B chunks of a key, or of a query, that a lane holds
   static constexpr int LPR = KD == 3 ? 16 : 4 * KD;  // bf16: lanes that read one row of V (12 of 16 at 96)
-  static constexpr int NV = kBf16 ? LPR / 2 : 2 * KD;  // bf16: 16-B loads of a block's V; f32: 16-B register groups
+  static constexpr int VT = kBf16 ? LPR / 4 : 2 * KD;  // 16-B loads (f32: register groups) of a tile's V
+  static constexpr int NV = KT * VT;
   static constexpr int PER = 64 / KT;                  // blocks whose page ids one load brings
   static constexpr int kOut = 1 << 30;
   using Q = uint4[NK];
@@ -190,13 +206,13 @@ struct Walk {
 
   // Queries: column c is row `out` of q. bf16: chunk k holds dims 32 k + 8 g .. + 7; f32: dims 16 k + 4 g .. + 3 (the
   // products contract over lane groups, in this permuted order on both sides).
-  __device__ __forceinline__ void load_q(Q& qf, const Row& r) const {
+  __device__ __forceinline__ void load_q(Q& qf, int64_t out, bool exists) const {
     constexpr int E = kBf16 ? 8 : 4;
-    const T* p = reinterpret_cast<const T*>(a.q) + (r.out * a.H + h) * a.hd;
+    const T* p = reinterpret_cast<const T*>(a.q) + (out * a.H + h) * a.hd;
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
       const int d = k * 4 * E + E * g;
-      qf[k] = (r.active && d < a.hd) ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
+      qf[k] = (exists && d < a.hd) ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
     }
   }
 
@@ -207,85 +223,86 @@ struct Walk {
     const int key = key_of(k0, stride);
     return k0 >= 0 && key < limit ? tab[key >> a.psl] : -1;
   }
-  __device__ __forceinline__ int check(int id, int k0, int stride, int k_end) const {
-    if (key_of(k0, stride) >= k_end) return -1;
-    if (id >= 0 && id < a.n_pages) return id;
-    set_err(a.err, ESGPT_FLAG_BAD_PAGE);
-    return -1;
+  // Byte offsets of the pages' rows that a walk up to k_end reads, worked out for all lanes at once; hi < 0: none.
+  struct Offsets {
+    int lo, hi;
+  };
+  __device__ __forceinline__ Offsets check(int id, int k0, int stride, int k_end) const {
+    const int key = key_of(k0, stride);
+    if (key >= k_end) return {0, -1};
+    if (id < 0 || id >= a.n_pages) {
+      set_err(a.err, ESGPT_FLAG_BAD_PAGE);
+      return {0, -1};
+    }
+    const int64_t off = ((((int64_t)id * a.H + h) << a.psl) + (key & ((1 << a.psl) - 1))) * (a.hd * (int)sizeof(T));
+    return {(int)off, (int)(off >> 32)};
   }
 
-  // A block's 16-row tiles in the pools: range-checked buffers that read zeros past k_end and on a bad page.
+  // A block's 16-row tiles: where they are in the pools and how many bytes of them a walk may read (none on a bad page).
   struct Tiles {
-    __amdgpu_buffer_rsrc_t k[KT], v[KT];
-    const T* vb[KT];
-    bool ok[KT];
+    int64_t off[KT];
+    int bytes[KT];
   };
-  __device__ __forceinline__ Tiles tiles(int k0, int k_end, int pid, int slot) const {
+  __device__ __forceinline__ Tiles tiles(int k0, int k_end, const Offsets& of, int slot) const {
     Tiles b;
+    const int rb = a.hd * (int)sizeof(T);
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      const int id = __builtin_amdgcn_readlane(pid, slot * KT + t);
-      b.ok[t] = id >= 0;
-      const int64_t row = b.ok[t] ? (((int64_t)id * a.H + h) << a.psl) + ((k0 + 16 * t) & ((1 << a.psl) - 1)) : 0;
-      const int n = b.ok[t] ? min(16, max(0, k_end - k0 - 16 * t)) * a.hd * (int)sizeof(T) : 0;
-      b.vb[t] = reinterpret_cast<const T*>(a.vp) + row * a.hd;
-      b.k[t] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(reinterpret_cast<const T*>(a.kp) + row * a.hd), (short)0,
-                                                 n, 0x00020000);
-      b.v[t] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(b.vb[t]), (short)0, n, 0x00020000);
+      const int hi = __builtin_amdgcn_readlane(of.hi, slot * KT + t);
+      const uint32_t lo = __builtin_amdgcn_readlane(of.lo, slot * KT + t);
+      b.off[t] = (int64_t)scalar(max(hi, 0)) << 32 | (uint32_t)scalar((int)lo);
+      b.bytes[t] = scalar(hi >= 0 ? min(16, max(0, k_end - k0 - 16 * t)) * rb : 0);
     }
     return b;
   }
+  // Range-checked buffers: rows past the end read as zeros.
+  __device__ __forceinline__ static __amdgpu_buffer_rsrc_t rows(const void* pool, int64_t off, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(pool) + off), (short)0, bytes,
+                                             0x00020000);
+  }
   __device__ __forceinline__ void load_k(uint4 (&k)[KT * NK], const Tiles& b) const {
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+    for (int t = 0; t < KT; ++t) {
+      const __amdgpu_buffer_rsrc_t r = rows(a.kp, b.off[t], b.bytes[t]);
 #pragma unroll
       for (int i = 0; i < NK; ++i)
-        k[t * NK + i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b.k[t], ko[i], 0, 0));
+        k[t * NK + i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, ko[i], 0, 0));
+    }
   }
   __device__ __forceinline__ void load_v(uint4 (&v)[NV], const Tiles& b) const {
     const int rb = a.hd * (int)sizeof(T);
-    if constexpr (kBf16) {
 #pragma unroll
-      for (int t = 0; t < KT; ++t)
+    for (int t = 0; t < KT; ++t) {
+      const __amdgpu_buffer_rsrc_t r = rows(a.vp, b.off[t], b.bytes[t]);
+      if constexpr (kBf16) {
 #pragma unroll
-        for (int i = 0; i < NV / 2; ++i)
-          v[t * (NV / 2) + i] = __builtin_bit_cast(
-              uint4, __builtin_amdgcn_raw_buffer_load_b128(b.v[t], vo[0] + i * (64 / LPR) * rb, 0, 0));
-    } else {
-      float2* f = reinterpret_cast<float2*>(v);
+        for (int i = 0; i < VT; ++i)
+          v[t * VT + i] =
+              __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, vo[0] + i * (64 / LPR) * rb, 0, 0));
+      } else {
+        float2* f = reinterpret_cast<float2*>(v + t * VT);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int p = 0; p < KD; ++p)
-          f[e * KD + p] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(b.v[0], vo[p] + e * rb, 0, 0));
-    }
-  }
-
-  __device__ __forceinline__ static bool nonfinite(const uint4 (&v)[NV]) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bad |= (w[j] & 0x7f800000u) == 0x7f800000u;
-        if (kBf16) bad |= (w[j] & 0x7f80u) == 0x7f80u;
+          for (int p = 0; p < KD; ++p)
+            f[e * KD + p] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(r, vo[p] + e * rb, 0, 0));
       }
     }
-    return bad;
   }
 
-  // P.V of a partly masked block whose values are not all finite, key by key: a key adds nothing (not even
-  // 0 x infinity) to the rows that do not see it. Rare: reads the values again.
-  __device__ __forceinline__ void masked_pv(const Tiles& b, const float (&p)[4 * KT], f32x4 (&o)[DT], int k0, int lo,
-                                            int hi) const {
+  // P.V of a partly masked block key by key: a key adds nothing (not even 0 x infinity) to the rows that do not see it.
+  // Reads the values again; only a walk that has met a value that is not finite comes here.
+  __device__ __forceinline__ void masked_pv(const Offsets& of, int slot, const float (&p)[4 * KT], f32x4 (&o)[DT], int k0,
+                                            int lo, int hi) const {
 #pragma nounroll
     for (int i = 0; i < 4 * KT; ++i) {
+      const int oh = __builtin_amdgcn_readlane(of.hi, slot * KT + (i >> 2));
+      if (oh < 0) continue;
+      const uint32_t ol = __builtin_amdgcn_readlane(of.lo, slot * KT + (i >> 2));
+      const T* vb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.vp) + ((int64_t)oh << 32 | ol));
       float pi = p[0];
 #pragma unroll
       for (int j = 1; j < 4 * KT; ++j) pi = i == j ? p[j] : pi;
-      if (!(i < 4 ? b.ok[0] : b.ok[KT - 1])) continue;
-      const T* vb = i < 4 ? b.vb[0] : b.vb[KT - 1];
 #pragma nounroll
       for (int gg = 0; gg < 4; ++gg) {
         const float pk = to_f32(from_f32<T>(__shfl(pi, 16 * gg + c, 64)));
@@ -302,45 +319,64 @@ struct Walk {
     }
   }
 
-  // Blocks k_first, k_first + stride, ... below k_end of the rows that tab names; raw: pages() of the first ones.
-  // Row (column c of tile t) sees keys [lo[t], hi[t]). k_first is a multiple of 16. A block's V goes to LDS at the top
-  // of its step and its K to the matrix units right after, and the next block's loads follow each: one set of
-  // registers, a whole step of latency covered.
-  template <int NT>
-  __device__ __forceinline__ void walk(State<NT, DT>& st, const Q (&qf)[NT], const int32_t* tab, int raw, int k_first,
-                                       int stride, int k_end, const int (&lo)[NT], const int (&hi)[NT],
-                                       const bool (&act)[NT]) const {
-    if (k_first >= k_end) return;
-    int lo_all = 0, hi_all = 0x7fffffff;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      if (act[t]) {
-        lo_all = max(lo_all, lo[t]);
-        hi_all = min(hi_all, hi[t]);
-      }
-    int pid = check(raw, k_first, stride, k_end), slot = 0;
-    Tiles b = tiles(k_first, k_end, pid, 0);
+  // A place in a walk: block k0 of segment seg, whose rows end at k_end; of: page offsets of the round of blocks that
+  // slot counts in.
+  struct At {
+    int seg, k0, k_end, slot;
+    Offsets of;
+  };
+  // Opens the first segment from `seg` on that has a key; false: none is left.
+  template <class Segs>
+  __device__ __forceinline__ bool open(Segs& sg, int seg, At& at) const {
+    for (; seg < sg.count; ++seg) {
+      int raw;
+      sg.open(*this, seg, at.k0, at.k_end, raw);
+      at.k0 = scalar(at.k0);
+      at.k_end = scalar(at.k_end);
+      if (at.k0 >= at.k_end) continue;
+      at.seg = seg;
+      at.slot = 0;
+      at.of = check(raw, at.k0, sg.stride(seg), at.k_end);
+      return true;
+    }
+    return false;
+  }
+  template <class Segs>
+  __device__ __forceinline__ bool next(Segs& sg, At& at) const {
+    const int stride = sg.stride(at.seg), k1 = at.k0 + stride;
+    if (k1 >= at.k_end) return open(sg, at.seg + 1, at);
+    at.k0 = k1;
+    if (++at.slot == PER) {
+      at.slot = 0;
+      at.of = check(pages(sg.table(at.seg), k1, stride, at.k_end), k1, stride, at.k_end);
+    }
+    return true;
+  }
+
+  // One pass over the segments of Segs (runs of keys with one page table and one set of limits each: row (column c of
+  // tile t) sees keys [lo[t], hi[t])), block by block. A block's V goes to LDS at the top of its step and its K to the
+  // matrix units right after, and the next block's loads (of the next segment, at a segment's end) follow each: one set
+  // of registers, a whole step of latency covered.
+  // exact: see masked_pv.
+  template <int NT, class Segs>
+  __device__ __forceinline__ void pass(State<NT, DT>& st, const Q (&qf)[NT], Segs& sg, bool exact) const {
+    At at;
+    if (!open(sg, 0, at)) return;
+    Tiles nb = tiles(at.k0, at.k_end, at.of, 0);
     uint4 k[KT * NK], v[NV];
-    load_k(k, b);
-    load_v(v, b);
-    lo_all = wave_max_i(lo_all);
-    hi_all = wave_min_i(hi_all);
-    for (int k0 = k_first;; k0 += stride) {
-      const int k1 = k0 + stride;
-      const bool more = k1 < k_end;
-      Tiles nb = b;
-      if (more) {
-        if (++slot == PER) {
-          slot = 0;
-          pid = check(pages(tab, k1, stride, k_end), k1, stride, k_end);
-        }
-        nb = tiles(k1, k_end, pid, slot);
-      }
-      bool full = k0 >= lo_all && k0 + KB <= hi_all && k0 + KB <= k_end;
+    load_k(k, nb);
+    load_v(v, nb);
+    int lo[NT], hi[NT], lo_all, hi_all, seg = -1;
+    for (;;) {
+      const At now = at;
+      const int k0 = at.k0;
+      uint32_t gone = 0;  // tiles without a row: a bad page, or past the end
 #pragma unroll
-      for (int t = 0; t < KT; ++t) full = full && b.ok[t];
-      bool slow = false;
-      if (!full) slow = __any(nonfinite(v));
+      for (int t = 0; t < KT; ++t) gone |= nb.bytes[t] == 0 ? 1u << t : 0u;
+      if (seg != at.seg) sg.limits(seg = at.seg, lo, hi, lo_all, hi_all);
+      const bool more = next(sg, at);
+      if (more) nb = tiles(at.k0, at.k_end, at.of, at.slot);
+      const bool full = k0 >= lo_all && k0 + KB <= hi_all && k0 + KB <= now.k_end && !gone;
       if constexpr (kBf16) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -363,7 +399,7 @@ struct Walk {
           } else {
 #pragma unroll
             for (int i = 0; i < 2 * KD; ++i) {
-              const f32x4 kf = __builtin_bit_cast(f32x4, k[i]), q4 = __builtin_bit_cast(f32x4, qf[t][i]);
+              const f32x4 kf = __builtin_bit_cast(f32x4, k[u * NK + i]), q4 = __builtin_bit_cast(f32x4, qf[t][i]);
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], q4[e], s[t][u], 0, 0, 0);
             }
@@ -374,11 +410,15 @@ struct Walk {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (!full) {
+          // a masked score is -inf (it may be NaN); its probability is then an exact zero
+          const int l0 = lo[t] - k0 - 4 * g;
+          const uint32_t span = (uint32_t)max(hi[t] - lo[t], 0);
 #pragma unroll
-          for (int i = 0; i < 4 * KT; ++i) {
-            const int key = k0 + 16 * (i >> 2) + 4 * g + (i & 3);
-            // a masked score is -inf (it may be NaN); its probability is then an exact zero
-            if (!(key >= lo[t] && key < hi[t] && b.ok[i >> 2])) s[t][i >> 2][i & 3] = -INFINITY;
+          for (int u = 0; u < KT; ++u) {
+            const uint32_t su = gone >> u & 1 ? 0u : span;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!((uint32_t)(16 * u + r - l0) < su)) s[t][u][r] = -INFINITY;
           }
         }
         float mx = s[t][0][0];
@@ -401,46 +441,71 @@ struct Walk {
         }
         st.l[t] += sum;
       }
-      if (slow) {
+      if (exact && !full) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) masked_pv(b, p[t], st.acc[t], k0, lo[t], hi[t]);
+        for (int t = 0; t < NT; ++t) masked_pv(now.of, now.slot, p[t], st.acc[t], k0, lo[t], hi[t]);
       } else if constexpr (kBf16) {
         // P in bf16 for the matrix product (as esgpt_attn_fwd and esgpt_attn_decode round it; the sums stay f32)
-        bf16x8 pf[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pf[t][i] = (__bf16)p[t][i];
         const __bf16* vr = vt + (4 * g + (c >> 2)) * LD + 4 * (c & 3);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          typedef __attribute__((address_space(3))) bf16x4* lds4;
-          const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * d));
-          const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * LD + 16 * d));
-          bf16x8 vf;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            vf[i] = x[i];
-            vf[4 + i] = y[i];
-          }
+        for (int u = 0; u < KT; u += 2) {
+          bf16x8 pf[NT];
 #pragma unroll
           for (int t = 0; t < NT; ++t)
-            st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], st.acc[t][d], 0, 0, 0);
-        }
-      } else {
-        const float* f = reinterpret_cast<const float*>(v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+            for (int i = 0; i < 8; ++i) pf[t][i] = (__bf16)p[t][4 * u + i];
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
+          for (int d = 0; d < DT; ++d) {
+            typedef __attribute__((address_space(3))) bf16x4* lds4;
+            const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * u * LD + 16 * d));
+            const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * (u + 1) * LD + 16 * d));
+            bf16x8 vf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              vf[i] = x[i];
+              vf[4 + i] = y[i];
+            }
 #pragma unroll
             for (int t = 0; t < NT; ++t)
-              st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[(e * KD + (d >> 1)) * 2 + (d & 1)], p[t][e],
-                                                                  st.acc[t][d], 0, 0, 0);
+              st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], st.acc[t][d], 0, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+          const float* f = reinterpret_cast<const float*>(v + u * VT);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+                st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[(e * KD + (d >> 1)) * 2 + (d & 1)], p[t][4 * u + e],
+                                                                    st.acc[t][d], 0, 0, 0);
+        }
       }
       if (!more) break;
       if constexpr (!kBf16) load_v(v, nb);
-      b = nb;
+    }
+  }
+
+  // A pass; where a sum is not finite, another that keeps such values from the rows that do not see them (0 x infinity
+  // would have reached the whole block's).
+  template <int NT, class Segs>
+  __device__ __forceinline__ void walk(State<NT, DT>& st, const Q (&qf)[NT], const Segs& segments) const {
+    for (bool exact = false;; exact = true) {
+      st.clear();
+      Segs sg = segments;
+      pass(st, qf, sg, exact);
+      if (exact) return;
+      float z = 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) z = fmaf(st.acc[t][d][r], 0.f, z);
+      if (!__any(z != 0.f)) return;
     }
   }
 };
@@ -481,7 +546,7 @@ struct Join {
   template <int NT>
   __device__ __forceinline__ static void run(const SharedArgs& a, const State<NT, 2 * KD>& st, int t, bool act, char* lds,
                                              int64_t out0, int r0, int h, int part) {
-    const int w = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, c = lane & 15;
+    const int w = scalar(threadIdx.x >> 6), lane = lane_id(), g = lane >> 4, c = lane & 15;
     float* jo = reinterpret_cast<float*>(lds);  // [wave][16][OLD]
     float* jm = jo + NW * 16 * OLD;             // [wave][16]
     float* jl = jm + NW * 16;
@@ -529,15 +594,56 @@ struct Join {
   }
 };
 
+// The limits that hold for every column that counts: blocks within them need no mask.
+template <int NT>
+__device__ __forceinline__ void common_limits(const int (&lo)[NT], const int (&hi)[NT], const bool (&act)[NT], int& lo_all,
+                                              int& hi_all) {
+  lo_all = 0;
+  hi_all = 0x7fffffff;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    if (act[t]) {
+      lo_all = max(lo_all, lo[t]);
+      hi_all = min(hi_all, hi[t]);
+    }
+  lo_all = cols_max(lo_all);
+  hi_all = cols_min(hi_all);
+}
+
+// One segment: a chunk of a history, or of one trajectory's own rows.
+template <int NT>
+struct OneSegment {
+  const int32_t* tab;
+  int first, end, step, raw, lo[NT], hi[NT];
+  bool act[NT];
+  static constexpr int count = 1;
+  __device__ __forceinline__ int stride(int) const { return step; }
+  __device__ __forceinline__ const int32_t* table(int) const { return tab; }
+  template <class W>
+  __device__ __forceinline__ void open(const W&, int, int& k0, int& k_end, int& ids) const {
+    k0 = first;
+    k_end = end;
+    ids = raw;
+  }
+  __device__ __forceinline__ void limits(int, int (&l)[NT], int (&u)[NT], int& lo_all, int& hi_all) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      l[t] = lo[t];
+      u[t] = hi[t];
+    }
+    common_limits<NT>(lo, hi, act, lo_all, hi_all);
+  }
+};
+
 // Split form: a workgroup per history chunk of one (group, head, 16 NT rows), then four waves a workgroup with the own
 // rows of one (trajectory, head, chunk) each.
 template <typename T, int KD, int NT>
-__global__ __launch_bounds__(64 * kWaves) void shared_kernel(SharedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, KD * NT < 8 ? 2 : 1) void shared_kernel(SharedArgs a) {
   using W = Walk<T, KD>;
   using J = Join<T, KD, kWaves>;
   constexpr int kTile = W::kBf16 ? W::KB * W::LD * 2 : 0;
   __shared__ __align__(16) char lds[(kWaves * kTile > J::kBytes) ? kWaves * kTile : J::kBytes];
-  const int w = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, c = lane & 15;
+  const int w = scalar(threadIdx.x >> 6), lane = lane_id(), g = lane >> 4, c = lane & 15;
 
   if ((int)blockIdx.x >= a.units) {
     // column c is the trajectory's new event c
@@ -545,20 +651,22 @@ __global__ __launch_bounds__(64 * kWaves) void shared_kernel(SharedArgs a) {
     const int ch = id % a.NSc, sh = id / a.NSc, h = sh % a.H, s = sh / a.H;
     if (s >= a.S) return;
     const W x(a, h, lds + w * kTile);
-    const int32_t* tab = a.table + (int64_t)s * a.table_w;
-    int raw = a.window ? -1 : x.pages(tab, ch * a.schunk, W::KB, a.cap);
-    const Row r = row_of(a, s, c, c < a.Lq);
+    OneSegment<1> sg;
+    sg.tab = a.table + (int64_t)s * a.table_w;
+    sg.step = W::KB;
+    sg.raw = a.window ? -1 : x.pages(sg.tab, ch * a.schunk, W::KB, a.cap);
     typename W::Q q[1];
-    x.load_q(q[0], r);
-    const int hi = r.active ? min(r.at + 1, a.cap) : 0, lo = (r.active && a.window) ? max(0, r.at - a.window + 1) : 0;
-    const int base = wave_min_i(r.active ? lo : a.cap) & ~15;  // no active row: no key
-    const int end = wave_max_i(hi), first = base + ch * a.schunk;
-    if (a.window && first < end) raw = x.pages(tab, first, W::KB, end);
+    x.load_q(q[0], (int64_t)s * a.Lq + c, c < a.Lq);
+    const Row r = row_of(a, s, c, c < a.Lq);
+    sg.act[0] = r.active;
+    sg.hi[0] = r.active ? min(r.at + 1, a.cap) : 0;
+    sg.lo[0] = (r.active && a.window) ? max(0, r.at - a.window + 1) : 0;
+    const int base = cols_min(r.active ? sg.lo[0] : a.cap) & ~15, end = cols_max(sg.hi[0]);  // no active row: no key
+    sg.first = base + ch * a.schunk;
+    sg.end = min(end, sg.first + a.schunk);
+    if (a.window && sg.first < sg.end) sg.raw = x.pages(sg.tab, sg.first, W::KB, sg.end);
     State<1, W::DT> st;
-    st.clear();
-    const int los[1] = {lo}, his[1] = {hi};
-    const bool act[1] = {r.active};
-    x.walk(st, q, tab, raw, first, W::KB, min(end, first + a.schunk), los, his, act);
+    x.walk(st, q, sg);
     const float l = r.active ? xsum(st.l[0]) : 0.f;
     if (c < a.Lq) {
 #pragma unroll
@@ -575,99 +683,118 @@ __global__ __launch_bounds__(64 * kWaves) void shared_kernel(SharedArgs a) {
   const int id = xcd_linear(blockIdx.x, a.units);
   const int rt = id % a.RT, ch = id / a.RT % a.NPc, gh = id / a.RT / a.NPc;
   const int h = gh % a.H, grp = gh / a.H;
+  const int64_t out0 = (int64_t)grp * a.M;
   const W x(a, h, lds + w * kTile);
-  const int32_t* tab = a.prefix_table + (int64_t)grp * a.prefix_w;
-  constexpr int kStride = kWaves * W::KB;
-  int raw = a.window ? -1 : x.pages(tab, ch * a.pchunk + w * W::KB, kStride, a.prefix_cap);
-  const int P = prefix_len(a, grp);
-  int lo[NT], hi[NT], base = a.prefix_cap;
-  bool act[NT];
+  OneSegment<NT> sg;
+  sg.tab = a.prefix_table + (int64_t)grp * a.prefix_w;
+  sg.step = kWaves * W::KB;
+  sg.raw = a.window ? -1 : x.pages(sg.tab, ch * a.pchunk + w * W::KB, sg.step, a.prefix_cap);
   typename W::Q q[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int rr = rt * 16 * NT + 16 * t + c;
+    x.load_q(q[t], out0 + rr, rr < a.M);
+  }
+  const int P = prefix_len(a, grp);
+  int base = a.prefix_cap;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int rr = rt * 16 * NT + 16 * t + c;
     const Row r = row_of(a, grp * a.n + rr / a.Lq, rr % a.Lq, rr < a.M);
-    x.load_q(q[t], r);
-    act[t] = r.active;
-    hi[t] = act[t] ? P : 0;
-    lo[t] = (act[t] && a.window) ? min(P, max(0, P + r.at - a.window + 1)) : 0;
-    if (act[t]) base = min(base, lo[t]);
+    sg.act[t] = r.active;
+    sg.hi[t] = r.active ? P : 0;
+    sg.lo[t] = (r.active && a.window) ? min(P, max(0, P + r.at - a.window + 1)) : 0;
+    if (r.active) base = min(base, sg.lo[t]);
   }
   // chunks count from the first row that a window of this group can reach, whatever its own rows
-  const int c0 = ((a.window ? max(0, P - a.window) : 0) & ~15) + ch * a.pchunk, end = min(P, c0 + a.pchunk);
-  int first = c0 + w * W::KB;
+  const int c0 = ((a.window ? max(0, P - a.window) : 0) & ~15) + ch * a.pchunk;
+  sg.end = min(P, c0 + a.pchunk);
+  sg.first = c0 + w * W::KB;
   if (a.window) {  // whole rounds of blocks before the first visible key
-    first += max(0, (wave_min_i(base) & ~15) - c0) / kStride * kStride;
-    if (first < end) raw = x.pages(tab, first, kStride, end);
+    sg.first += max(0, (cols_min(base) & ~15) - c0) / sg.step * sg.step;
+    if (sg.first < sg.end) sg.raw = x.pages(sg.tab, sg.first, sg.step, sg.end);
   }
   State<NT, W::DT> st;
-  st.clear();
-  x.walk(st, q, tab, raw, first, kStride, end, lo, hi, act);
-  const int64_t out0 = (int64_t)grp * a.M;
-  J::run(a, st, 0, act[0], lds, out0, rt * 16 * NT, h, ch);
-  if constexpr (NT == 2) J::run(a, st, 1, act[1], lds, out0, rt * 16 * NT + 16, h, ch);
+  x.walk(st, q, sg);
+  J::run(a, st, 0, sg.act[0], lds, out0, rt * 16 * NT, h, ch);
+  if constexpr (NT == 2) J::run(a, st, 1, sg.act[1], lds, out0, rt * 16 * NT + 16, h, ch);
 }
 
 // Whole form: one workgroup of NW waves per (group, head, 16 rows) does the rows' history and their own rows and writes
-// the result. The waves take every NW-th block of the history and, from the other end, every NW-th trajectory.
+// the result. The waves take every NW-th block of the history (segment 0) and, from the other end, every NW-th
+// trajectory's own rows, which only that trajectory's columns see; a segment's page ids are loaded when the one before is
+// opened.
 template <typename T, int KD, int NW>
 __global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
   using W = Walk<T, KD>;
   using J = Join<T, KD, NW>;
   constexpr int kTile = W::kBf16 ? W::KB * W::LD * 2 : 0;
   __shared__ __align__(16) char lds[(NW * kTile > J::kBytes) ? NW * kTile : J::kBytes];
-  const int w = threadIdx.x >> 6, lane = lane_id(), c = lane & 15;
+  const int w = scalar(threadIdx.x >> 6), lane = lane_id(), c = lane & 15;
   const int id = xcd_linear(blockIdx.x, gridDim.x);
   const int rt = id % a.RT, gh = id / a.RT, h = gh % a.H, grp = gh / a.H;
+  const int64_t out0 = (int64_t)grp * a.M;
   const W x(a, h, lds + w * kTile);
-  const int32_t* ptab = a.prefix_table + (int64_t)grp * a.prefix_w;
-  constexpr int kStride = NW * W::KB;
-  const int rr = rt * 16 + c;
-  const int s0 = grp * a.n + rt * 16 / a.Lq, ns = grp * a.n + min(a.M - 1, rt * 16 + 15) / a.Lq - s0 + 1;
-  const int ow = NW - 1 - w;
-  // page ids that need no length: of the history, and of this wave's first trajectory
-  int raw = a.window ? -1 : x.pages(ptab, w * W::KB, kStride, a.prefix_cap);
-  int oraw = a.window || ow >= ns ? -1 : x.pages(a.table + (int64_t)(s0 + ow) * a.table_w, 0, W::KB, a.cap);
-  const int P = prefix_len(a, grp);
-  const int my = grp * a.n + rr / a.Lq;  // this column's trajectory
-  const Row r = row_of(a, my, rr % a.Lq, rr < a.M);
+
+  struct Segs {
+    const SharedArgs& a;
+    const int32_t* ptab;
+    int w, s0, count, P, my, plo, phi, olo, ohi, ids;
+    bool act;
+    __device__ __forceinline__ int seq(int seg) const { return s0 + (NW - 1 - w) + (seg - 1) * NW; }
+    __device__ __forceinline__ int stride(int seg) const { return seg == 0 ? NW * W::KB : W::KB; }
+    __device__ __forceinline__ const int32_t* table(int seg) const {
+      return seg == 0 ? ptab : a.table + (int64_t)seq(seg) * a.table_w;
+    }
+    __device__ __forceinline__ void open(const W& x, int seg, int& k0, int& k_end, int& raw) {
+      raw = ids;
+      if (seg == 0) {
+        k0 = w * W::KB + (cols_min(act ? plo : P) & ~15);
+        k_end = P;
+      } else {
+        const bool mine = act && my == seq(seg);
+        k0 = cols_min(mine ? olo : a.cap) & ~15;
+        k_end = cols_max(mine ? ohi : 0);
+      }
+      if (a.window) {
+        if (k0 < k_end) raw = x.pages(table(seg), k0, stride(seg), k_end);
+      } else if (seg + 1 < count) {
+        ids = x.pages(table(seg + 1), 0, W::KB, a.cap);
+      }
+    }
+    __device__ __forceinline__ void limits(int seg, int (&lo)[1], int (&hi)[1], int& lo_all, int& hi_all) const {
+      if (seg == 0) {
+        lo[0] = plo;
+        hi[0] = phi;
+        const bool on[1] = {act};
+        common_limits<1>(lo, hi, on, lo_all, hi_all);
+      } else {  // the other trajectories' columns see none of these rows
+        const bool mine = act && my == seq(seg);
+        lo[0] = olo;
+        hi[0] = mine ? ohi : 0;
+        lo_all = hi_all = 0;
+      }
+    }
+  };
+
+  const int rr = rt * 16 + c, s0 = grp * a.n + rt * 16 / a.Lq;
+  const int ns = grp * a.n + min(a.M - 1, rt * 16 + 15) / a.Lq - s0 + 1;
+  Segs sg{a, a.prefix_table + (int64_t)grp * a.prefix_w, w, s0, 1 + max(0, (ns - (NW - 1 - w) + NW - 1) / NW)};
+  sg.ids = a.window ? -1 : x.pages(sg.ptab, w * W::KB, sg.stride(0), a.prefix_cap);
   typename W::Q q[1];
-  x.load_q(q[0], r);
+  x.load_q(q[0], out0 + rr, rr < a.M);
+  sg.P = prefix_len(a, grp);
+  sg.my = grp * a.n + rr / a.Lq;  // this column's trajectory
+  const Row r = row_of(a, sg.my, rr % a.Lq, rr < a.M);
+  sg.act = r.active;
+  const bool cut = r.active && a.window;
+  sg.phi = r.active ? sg.P : 0;
+  sg.plo = cut ? min(sg.P, max(0, sg.P + r.at - a.window + 1)) : 0;
+  sg.ohi = r.active ? min(r.at + 1, a.cap) : 0;
+  sg.olo = cut ? max(0, r.at - a.window + 1) : 0;
   State<1, W::DT> st;
-  st.clear();
-  {
-    const int lo[1] = {(r.active && a.window) ? min(P, max(0, P + r.at - a.window + 1)) : 0}, hi[1] = {r.active ? P : 0};
-    const bool act[1] = {r.active};
-    int first = w * W::KB;
-    if (a.window) {
-      first += wave_min_i(r.active ? lo[0] : P) & ~15;
-      if (first < P) raw = x.pages(ptab, first, kStride, P);
-    }
-    x.walk(st, q, ptab, raw, first, kStride, P, lo, hi, act);
-  }
-  for (int j = ow; j < ns; j += NW) {
-    const int s = s0 + j;
-    const int32_t* tab = a.table + (int64_t)s * a.table_w;
-    const bool act[1] = {r.active && my == s};
-    const int lo[1] = {(act[0] && a.window) ? max(0, r.at - a.window + 1) : 0}, hi[1] = {act[0] ? min(r.at + 1, a.cap) : 0};
-    const int first = wave_min_i(act[0] ? lo[0] : a.cap) & ~15, end = wave_max_i(hi[0]);
-    if (first >= end) continue;
-    if (a.window || j != ow) oraw = x.pages(tab, first, W::KB, end);
-    State<1, W::DT> own;
-    own.clear();
-    x.walk(own, q, tab, oraw, first, W::KB, end, lo, hi, act);
-    // into this wave's state, the trajectory's columns only
-    const float mn = fmaxf(st.m[0], own.m[0]), mc = mn == -INFINITY ? 0.f : mn * kLog2e;
-    const float fa = __builtin_amdgcn_exp2f(fmaf(st.m[0], kLog2e, -mc));
-    const float fb = __builtin_amdgcn_exp2f(fmaf(own.m[0], kLog2e, -mc));
-    if (act[0]) {
-      st.m[0] = mn;
-      st.l[0] = fmaf(st.l[0], fa, own.l[0] * fb);
-#pragma unroll
-      for (int d = 0; d < W::DT; ++d) st.acc[0][d] = st.acc[0][d] * fa + own.acc[0][d] * fb;
-    }
-  }
-  J::run(a, st, 0, r.active, lds, (int64_t)grp * a.M, rt * 16, h, 0);
+  x.walk(st, q, sg);
+  J::run(a, st, 0, r.active, lds, out0, rt * 16, h, 0);
 }
 
 // Joins a row's parts: o = sum_p e^{m_p - M} O_p / sum_p e^{m_p - M} l_p. One wave per (row, head): lane groups of
@@ -713,36 +840,50 @@ struct SharedPlan {
 
 // Waves of the whole form's workgroup: past 64 dimensions a wave's registers and LDS leave room for four.
 int whole_waves(int64_t hd) { return hd <= 64 ? 8 : 4; }
-constexpr int64_t kWholeSteps = 8, kWholeUnits = 1024;
+// Keys of one block of a walk (Walk::KB).
+int block_keys(int64_t hd, int dtype) {
+  return dtype == ESGPT_BF16 ? (hd <= 64 ? Walk<bf16, 2>::KB : Walk<bf16, 4>::KB)
+                             : (hd <= 64 ? Walk<float, 2>::KB : Walk<float, 4>::KB);
+}
 
+// Whole or split. The whole form saves the second launch and the parts' traffic but has 16 rows' keys on one CU; what it
+// costs is its busiest wave's chain of blocks (steps: those of the history and those of its trajectories' own rows).
+// Measured in graph replays, whole / split us (groups x trajectories, history + own rows, heads, head size):
+//   every block and trajectory has a wave of its own: 8x4 100+10 h4 hd64 bf16 6.7 / 7.9; 1x4 40+6 f32 hd16 6.3 / 7.1
+//     (not so: 4x8 200+20 f32 8.6 / 7.6)
+//   half the CUs or more have a workgroup, three steps: 32x16 256+64 h4 13.1 / 14.8 (64 workgroups, 16x4 1024+32: 12.8 / 11.5)
+//   one workgroup per CU or more: 32x8 512+24 window 32 9.2 / 14.4; 64x4 300+20 11.3 / 12.4; 32x16 2048+32 h8 35.5 / 39.3;
+//     unless the own rows are the longer chain: 64x1 512+400 34.9 / 24.9.
+// The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 55.8 / 58.8, 8x8 8192+32 f32 50.7 /
+// 52.2, 16x4 1024+33 f32 15.0 / 18.2, 4x64 2048+32 16.9 / 20.1 (more parts cost more joins); own rows at 1,024 waves: 16x16
+// 256+64 f32 15.7 against 19.7 at 4,096.
 SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap, int64_t cap,
                        int64_t window, int dtype) {
   SharedPlan p;
-  const int64_t M = (S / G) * Lq, kb = dtype == ESGPT_BF16 ? 32 : 16;
+  constexpr int64_t kCus = 256;
+  const int64_t M = (S / G) * Lq, kb = block_keys(hd, dtype), nw = whole_waves(hd);
   const int64_t pspan = window ? std::min(prefix_cap, window + 16) : prefix_cap;
   const int64_t sspan = window ? std::min(cap, window + Lq + 16) : cap;
-  {
-    // whole form: blocks of keys that its busiest wave walks one after the other
-    const int64_t seqs = std::min<int64_t>(cdiv(std::min<int64_t>(M, 16), Lq) + (Lq > 1), S / G);
-    const int64_t nw = whole_waves(hd), steps = cdiv(pspan, nw * kb) + cdiv(seqs, nw) * cdiv(sspan, kb);
-    p.RT = (int)cdiv(M, 16);
-    p.units = G * H * p.RT;
-    p.whole = steps <= kWholeSteps || p.units >= kWholeUnits;
-    if (p.whole) {
-      p.NT = p.NP = 1;
-      p.NPc = p.NSc = p.pchunk = p.schunk = 0;
-      p.own_blocks = 0;
-      return p;
-    }
+  const int64_t seqs = std::min<int64_t>(cdiv(std::min<int64_t>(M, 16), Lq) + (Lq > 1), S / G);  // of 16 rows
+  const int64_t steps = cdiv(pspan, nw * kb), own_steps = cdiv(seqs, nw) * cdiv(sspan, kb);
+  p.RT = (int)cdiv(M, 16);
+  p.units = G * H * p.RT;
+  p.whole = cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw || (p.units >= kCus / 2 && steps + own_steps <= 3) ||
+            (p.units >= kCus && own_steps <= std::max<int64_t>(4, steps));
+  if (p.whole) {
+    p.NT = p.NP = 1;
+    p.NPc = p.NSc = p.pchunk = p.schunk = 0;
+    p.own_blocks = 0;
+    return p;
   }
   p.NT = dtype == ESGPT_BF16 && M > 16 ? 2 : 1;
   p.RT = (int)cdiv(M, 16 * p.NT);
   const int64_t round = kWaves * kb;
   const int64_t base = G * H * p.RT;
-  p.NPc = pspan ? (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, base), cdiv(pspan, round), 48})) : 0;
+  p.NPc = pspan ? (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(kCus, base), cdiv(pspan, round), 48})) : 0;
   p.pchunk = p.NPc ? (int)(cdiv(cdiv(pspan, p.NPc), round) * round) : 0;
   p.NPc = p.NPc ? (int)cdiv(pspan, p.pchunk) : 0;
-  p.NSc = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(4096, S * H), cdiv(sspan, 2 * kb), 16}));
+  p.NSc = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(4 * kCus, S * H), cdiv(sspan, 2 * kb), 16}));
   p.schunk = (int)(cdiv(cdiv(sspan, p.NSc), kb) * kb);
   p.NSc = (int)cdiv(sspan, p.schunk);
   p.NP = p.NPc + p.NSc;

@@ -140,6 +140,10 @@ CASES = [
     (2, 3, 1, 2, 64, 64, 90, 20, 100000),
     (1, 6, 1, 2, 64, 64, 9001, 700, 0),  # many parts of a row
     (1, 2, 1, 1, 64, 16, 500, 3000, 0), (1, 40, 2, 1, 64, 64, 5000, 40, 700),
+    # enough (group, head)s for one workgroup each to do history and own rows in one launch
+    (16, 9, 1, 8, 64, 32, 100, 40, 0), (32, 3, 2, 4, 128, 16, 70, 20, 0), (16, 3, 1, 8, 96, 16, 90, 12, 20),
+    (33, 2, 1, 8, 40, 16, 20, 5, 0), (32, 20, 1, 4, 24, 16, 33, 9, 0), (32, 2, 5, 8, 16, 16, 600, 70, 0),
+    (64, 1, 1, 4, 64, 64, 20, 400, 0),
 ]
 
 
@@ -154,8 +158,8 @@ def test_against_the_oracle(c, dt):
 
 @gpu
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("c", [(64, 1, 1, 16, 16, 64, 4500, 3, 0), (300, 1, 1, 16, 16, 64, 3, 1300, 0),
-                               (64, 20, 1, 16, 16, 32, 4200, 2, 0)], ids=str)
+@pytest.mark.parametrize("c", [(64, 1, 1, 16, 16, 64, 4500, 1300, 0), (64, 1, 1, 16, 16, 64, 9000, 1100, 0),
+                               (64, 20, 1, 16, 16, 32, 8300, 2, 0), (300, 1, 1, 16, 16, 64, 3, 2300, 0)], ids=str)
 def test_more_keys_in_a_part_than_a_round_of_page_ids(c, dt):
     """Enough workgroups that a history (or own) part is longer than 64 page ids reach; all sequences name the same
     pages. The first sequences and the last one are checked."""
