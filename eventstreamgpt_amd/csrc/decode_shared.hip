@@ -854,6 +854,7 @@ int block_keys(int64_t hd, int dtype) {
 //   half the CUs or more have a workgroup, three steps: 32x16 256+64 h4 13.1 / 14.8 (64 workgroups, 16x4 1024+32: 12.8 / 11.5)
 //   one workgroup per CU or more: 32x8 512+24 window 32 9.2 / 14.4; 64x4 300+20 11.3 / 12.4; 32x16 2048+32 h8 35.5 / 39.3;
 //     unless the own rows are the longer chain: 64x1 512+400 34.9 / 24.9.
+// Without a history the split form's waves are the whole of it, and write directly where one chunk holds a trajectory.
 // The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 55.8 / 58.8, 8x8 8192+32 f32 50.7 /
 // 52.2, 16x4 1024+33 f32 15.0 / 18.2, 4x64 2048+32 16.9 / 20.1 (more parts cost more joins); own rows at 1,024 waves: 16x16
 // 256+64 f32 15.7 against 19.7 at 4,096.
@@ -868,8 +869,9 @@ SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, 
   const int64_t steps = cdiv(pspan, nw * kb), own_steps = cdiv(seqs, nw) * cdiv(sspan, kb);
   p.RT = (int)cdiv(M, 16);
   p.units = G * H * p.RT;
-  p.whole = cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw || (p.units >= kCus / 2 && steps + own_steps <= 3) ||
-            (p.units >= kCus && own_steps <= std::max<int64_t>(4, steps));
+  p.whole = pspan > 0 &&
+            (cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw || (p.units >= kCus / 2 && steps + own_steps <= 3) ||
+             (p.units >= kCus && own_steps <= std::max<int64_t>(4, steps)));
   if (p.whole) {
     p.NT = p.NP = 1;
     p.NPc = p.NSc = p.pchunk = p.schunk = 0;
@@ -959,13 +961,17 @@ int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_p
   if (S == 0 && Lq >= 0 && Lq <= kMaxLq) return ESGPT_OK;
   ESGPT_REQUIRE(shared_ok(G, S, Lq, H, hd, prefix_cap, cap, window, dtype));
   ESGPT_REQUIRE(page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0 && n_pages >= 0 &&
-                n_pages < (int64_t)1 << 31 && cap <= table_w * page_size && prefix_cap <= prefix_w * page_size);
+                n_pages < (int64_t)1 << 31 && table_w >= 0 && table_w < (int64_t)1 << 31 && prefix_w >= 0 &&
+                prefix_w < (int64_t)1 << 31 && cap <= table_w * page_size && prefix_cap <= prefix_w * page_size);
   auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
   ESGPT_REQUIRE(q && o && past && page_table && aligned(q) && aligned(o) && (prefix_cap == 0 || (prefix_table && prefix_lens)));
   ESGPT_REQUIRE(n_pages == 0 || (k_pages && v_pages && aligned(k_pages) && aligned(v_pages)));
   window = std::min<int64_t>(window, (int64_t)1 << 30);
   const SharedPlan p = shared_plan(G, S, Lq, H, hd, prefix_cap, cap, window, dtype);
-  ESGPT_REQUIRE(p.units + p.own_blocks < (int64_t)1 << 31);
+  // a launch holds fewer than 2^32 threads
+  constexpr int64_t kThreads = ((int64_t)1 << 32) - 1;
+  ESGPT_REQUIRE((p.units + p.own_blocks) * 64 * (p.whole ? whole_waves(hd) : kWaves) <= kThreads &&
+                cdiv(S * Lq * H, 4) * 256 <= kThreads);
   SharedArgs a{};
   if (p.NP > 1) {
     const size_t rows = (size_t)(S * Lq * H * p.NP);

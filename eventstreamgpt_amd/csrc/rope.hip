@@ -545,7 +545,7 @@ int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, c
   ESGPT_REQUIRE(S >= 0 && Lq >= 0 && Lq <= kTop && S <= kTop && S * Lq <= kTop);
   ESGPT_REQUIRE(rope_ok(qkv, q_w, k_w, pos, pos_dtype, inv_freq, R, S * Lq, H, hd, eps, dtype));
   ESGPT_REQUIRE(page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0 && table_w >= 0 &&
-                n_pages >= 0);
+                table_w < (int64_t)1 << 31 && n_pages >= 0 && n_pages < (int64_t)1 << 31);
   if (S * Lq == 0) return ESGPT_OK;
   ESGPT_REQUIRE(past && q && aligned16(q) && (table_w == 0 || page_table) &&
                 (n_pages == 0 || (k_pages && v_pages && aligned16(k_pages) && aligned16(v_pages))));

@@ -639,10 +639,11 @@ void check_pages(const char* what, const Tensor& like, const Tensor& k_pages, co
               " is not a power of two from 16 to 65536");
 }
 
-void check_i32(const char* what, const char* name, const Tensor& t, const Tensor& like, int64_t dim, int64_t rows) {
-  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.size(0) == rows && t.is_contiguous() &&
-                  t.device() == like.device(),
-              what, ": ", name, " must be a contiguous int32 tensor with ", rows, " rows on the device of the rows");
+// Page tables, lengths: int32 on the device (a slice of a wider table is copied).
+Tensor i32(const char* what, const char* name, const Tensor& t, const Tensor& like, int64_t dim, int64_t rows) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.size(0) == rows && t.device() == like.device(), what,
+              ": ", name, " must be an int32 tensor with ", rows, " rows on the device of the rows");
+  return t.contiguous();
 }
 
 Tensor row_mask_of(const char* what, const optional<Tensor>& m, const Tensor& like, int64_t S, int64_t Lq) {
@@ -659,8 +660,8 @@ int32_t* err_of(const char* what, const Tensor& err, const Tensor& like) {
   return reinterpret_cast<int32_t*>(err.data_ptr());
 }
 
-Tensor kv_append_paged(const Tensor& qkv_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
-                       const Tensor& past, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
+Tensor kv_append_paged(const Tensor& qkv_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table_,
+                       const Tensor& past_, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
                        const optional<Tensor>& k_w, const optional<Tensor>& pos, const optional<Tensor>& inv_freq,
                        double eps, const Tensor& err) {
   const char* what = "esgpt.kv_append_paged";
@@ -669,8 +670,7 @@ Tensor kv_append_paged(const Tensor& qkv_, const Tensor& k_pages, const Tensor& 
   TORCH_CHECK(hd == k_pages.size(3), what, ": the pages hold heads of ", k_pages.size(3), ", qkv of ", hd);
   const c10::DeviceGuard guard(qkv_.device());
   const RopeIn r = rope_in(what, qkv_, S, Lq, hd, q_w, k_w, pos, inv_freq);
-  check_i32(what, "page_table", page_table, qkv_, 2, S);
-  check_i32(what, "past", past, qkv_, 1, S);
+  const Tensor page_table = i32(what, "page_table", page_table_, qkv_, 2, S), past = i32(what, "past", past_, qkv_, 1, S);
   Tensor m = row_mask_of(what, row_mask, qkv_, S, Lq);
   int32_t* e = err_of(what, err, qkv_);
   Tensor qkv = rows16(qkv_);
@@ -686,7 +686,7 @@ Tensor kv_append_paged(const Tensor& qkv_, const Tensor& k_pages, const Tensor& 
 
 Tensor attn_decode_shared(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages,
                           const optional<Tensor>& prefix_table, const optional<Tensor>& prefix_lens,
-                          const Tensor& page_table, const Tensor& past, const optional<Tensor>& row_mask,
+                          const Tensor& page_table_, const Tensor& past_, const optional<Tensor>& row_mask,
                           int64_t prefix_cap, int64_t cap, int64_t window, const Tensor& err) {
   const char* what = "esgpt.attn_decode_shared";
   check_pages(what, q_, k_pages, v_pages);
@@ -699,15 +699,15 @@ Tensor attn_decode_shared(const Tensor& q_, const Tensor& k_pages, const Tensor&
   TORCH_CHECK(pre == (prefix_lens.has_value() && prefix_lens->defined()) && (pre || prefix_cap == 0), what,
               ": prefix_table and prefix_lens are given together, or not at all with prefix_cap = 0");
   const int64_t G = pre ? prefix_table->size(0) : S;
+  Tensor ptab, plen;
   if (pre) {
-    check_i32(what, "prefix_table", *prefix_table, q_, 2, G);
-    check_i32(what, "prefix_lens", *prefix_lens, q_, 1, G);
+    ptab = i32(what, "prefix_table", *prefix_table, q_, 2, G);
+    plen = i32(what, "prefix_lens", *prefix_lens, q_, 1, G);
     TORCH_CHECK(G > 0 ? S % G == 0 : S == 0, what, ": ", S, " sequences do not divide into ", G, " groups");
     TORCH_CHECK(prefix_cap >= 0 && prefix_cap <= prefix_table->size(1) * ps, what, ": prefix_cap = ", prefix_cap,
                 " is beyond the ", prefix_table->size(1) * ps, " rows of prefix_table");
   }
-  check_i32(what, "page_table", page_table, q_, 2, S);
-  check_i32(what, "past", past, q_, 1, S);
+  const Tensor page_table = i32(what, "page_table", page_table_, q_, 2, S), past = i32(what, "past", past_, q_, 1, S);
   TORCH_CHECK(cap >= 1 && cap <= page_table.size(1) * ps, what, ": cap = ", cap, " is not within the ",
               page_table.size(1) * ps, " rows of page_table");
   TORCH_CHECK(window >= 0, what, ": window = ", window);
@@ -720,8 +720,7 @@ Tensor attn_decode_shared(const Tensor& q_, const Tensor& k_pages, const Tensor&
   const size_t nb = esgpt_attn_decode_shared_workspace(G, S, Lq, H, hd, prefix_cap, cap, window, dt);
   Tensor ws = at::empty({(int64_t)nb}, q.options().dtype(at::kByte));
   check(esgpt_attn_decode_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.size(0), ps,
-                                 pre ? ptr<const int32_t>(*prefix_table) : nullptr, pre ? prefix_table->size(1) : 0,
-                                 pre ? ptr<const int32_t>(*prefix_lens) : nullptr, G, ptr<const int32_t>(page_table),
+                                 ptr<const int32_t>(ptab), pre ? ptab.size(1) : 0, ptr<const int32_t>(plen), G, ptr<const int32_t>(page_table),
                                  page_table.size(1), ptr<const int32_t>(past),
                                  m.defined() ? ptr<const uint8_t>(m) : nullptr, o.data_ptr(), S, Lq, H, hd, prefix_cap,
                                  cap, window, dt, ws.data_ptr(), nb, e, stream_of(q)),

@@ -554,6 +554,16 @@ def attention(qkv, key_mask, query_mask, H: int, window: int, static_kv_first: b
     return o
 
 
+def qk_norm_rope(qkv, q_w, k_w, pos, inv_freq, H: int, eps: float = 1e-6):
+    """``esgpt::qk_norm_rope``: packed ``qkv`` [Bs, T, 3D] -> the same with every head of q and k RMS-normalised (times
+    ``q_w`` / ``k_w`` [head size]; both None: not) and rotated by ``pos`` [Bs, T] * ``inv_freq`` (both None: not), what
+    ``attention`` reads. Differentiable in ``qkv``, ``q_w`` and ``k_w``."""
+    if qkv.device.type != "cuda":
+        raise L.HipExtensionMissing("eventstreamgpt_amd: qk_norm_rope needs a HIP device tensor (no CPU path)")
+    with _timed("qk_norm_rope"):
+        return _ops().qk_norm_rope(qkv, q_w, k_w, pos, inv_freq, int(H), float(eps))
+
+
 class AttentionFn:
     """Call-compatible name of ``attention`` (``AttentionFn.apply(qkv, key_mask, query_mask, H, window, skf, p)``)."""
 
@@ -649,10 +659,22 @@ def cached_attention(qkv: torch.Tensor, layer_past, key_mask: torch.Tensor | Non
 # Generation: paged cache with a shared history (csrc/rope.hip, csrc/decode_shared.hip)
 # ----------------------------------------------------------------------------------------------------------------
 class PagedKV:
-    """One layer's pool of cache pages for ``esgpt::kv_append_paged`` and ``esgpt::attn_decode_shared``: ``k`` / ``v``
-    [n_pages, H, page_size, head size], and the list of free pages. ``pages(count)`` hands out page ids (one row of a
-    page table, int32 on the device) and ``release(ids)`` takes them back; which sequence a page belongs to, and how
-    many of its rows are filled, is the caller's (page tables and ``past`` are plain tensors)."""
+    """One layer's pool of cache pages: ``k`` / ``v`` [n_pages, H, page_size, head size] and the list of free pages.
+
+    ``pages(count)`` hands out page ids (one row of a page table, int32 on the device) and ``release(ids)`` takes them
+    back; which sequence a page belongs to, and how many of its rows are filled, is the caller's (page tables and ``past``
+    are plain int32 tensors, and every layer of a step shares them). ``append`` stores new rows
+    (``esgpt::kv_append_paged``) and ``attend`` attends them (``esgpt::attn_decode_shared``). A generation with ``n``
+    trajectories per subject stores each subject's history once, under ``prefix_table``::
+
+        q = cache.append(history_qkv, prefix_table, zero, row_mask=event_mask, ...)     # [B, L, 3D], once
+        for each new event:                                                              # [B * n, 1, 3D]
+            q = cache.append(qkv, page_table, past, ...)
+            o = cache.attend(q, page_table, past, cap, prefix_table, event_mask.sum(1).int(), L)
+            past += 1                                                                    # after the last layer
+
+    A page id outside the pool or a length outside its table or bound raises ``IndexError`` at the next
+    ``check_errors()``; what has no place is not stored and not read."""
 
     def __init__(self, n_pages: int, page_size: int, H: int, head_size: int, dtype, device):
         if page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
@@ -672,6 +694,32 @@ class PagedKV:
         if len(set(ids)) != len(ids) or not all(0 <= i < self.k.shape[0] for i in ids) or set(ids) & set(self._free):
             raise ValueError(f"pages {ids} are not handed out (each once)")
         self._free.extend(ids)
+
+    def _usable(self, rows: torch.Tensor) -> None:
+        if torch.is_grad_enabled() and rows.requires_grad:
+            raise NotImplementedError("eventstreamgpt_amd: the KV-cache path is for generation (run under torch.no_grad())")
+        if rows.device.type != "cuda":
+            raise L.HipExtensionMissing("eventstreamgpt_amd: KV-cache attention needs a HIP device tensor")
+
+    def append(self, qkv, page_table, past, row_mask=None, q_w=None, k_w=None, pos=None, inv_freq=None,
+               eps: float = 1e-6) -> torch.Tensor:
+        """Stores the keys and values of packed ``qkv`` [S, Lq, 3D] behind each sequence's ``past`` rows, padded rows
+        (``row_mask`` False) left out; with ``q_w`` / ``k_w`` normalised and with ``pos`` / ``inv_freq`` rotated as
+        ``esgpt::qk_norm_rope`` does. Returns the queries [S, Lq, D], treated the same."""
+        self._usable(qkv)
+        with _timed("kv_append"):
+            return _ops().kv_append_paged(qkv, self.k, self.v, page_table, past, row_mask, q_w, k_w, pos, inv_freq,
+                                          float(eps), err_word(qkv.device))
+
+    def attend(self, q, page_table, past, cap: int, prefix_table=None, prefix_lens=None, prefix_cap: int = 0,
+               row_mask=None, window: int = 0) -> torch.Tensor:
+        """Causal (``window``: local) attention of the new events ``q`` [S, Lq, D], Lq <= 16, over their sequence's rows,
+        themselves included, and the history of their group; ``past`` and ``row_mask`` as ``append`` had them. ``cap`` /
+        ``prefix_cap`` bound past + new rows and ``prefix_lens`` (the closer, the better the work is split)."""
+        self._usable(q)
+        with _timed("attn_decode"):
+            return _ops().attn_decode_shared(q, self.k, self.v, prefix_table, prefix_lens, page_table, past, row_mask,
+                                             int(prefix_cap), int(cap), int(window), err_word(q.device))
 
 
 # ----------------------------------------------------------------------------------------------------------------

@@ -143,7 +143,7 @@ CASES = [
     # enough (group, head)s for one workgroup each to do history and own rows in one launch
     (16, 9, 1, 8, 64, 32, 100, 40, 0), (32, 3, 2, 4, 128, 16, 70, 20, 0), (16, 3, 1, 8, 96, 16, 90, 12, 20),
     (33, 2, 1, 8, 40, 16, 20, 5, 0), (32, 20, 1, 4, 24, 16, 33, 9, 0), (32, 2, 5, 8, 16, 16, 600, 70, 0),
-    (64, 1, 1, 4, 64, 64, 20, 400, 0),
+    (64, 1, 1, 4, 64, 64, 20, 400, 0), (1, 100, 1, 1, 64, 64, 90, 12, 0), (70, 1, 1, 4, 64, 16, 0, 90, 0),
 ]
 
 
@@ -400,11 +400,10 @@ def test_prompt_then_generation(dt, window):
     whole = torch.cat([hist.repeat_interleave(n, 0), new], 1)
     times = torch.cat([t_hist.repeat_interleave(n, 0), t_new], 1)
     keys = torch.cat([mask.repeat_interleave(n, 0), torch.ones(S, T, dtype=torch.bool, device=DEV)], 1)
-    y = ops().qk_norm_rope(whole, *w, times, f, H, 1e-6)
+    y = K.qk_norm_rope(whole, *w, times, f, H)
     for i in range(T):
-        q = ops().kv_append_paged(new[:, i: i + 1].contiguous(), cache.k, cache.v, table, past, None, *w, t_new[:, i: i + 1],
-                                  f, 1e-6, err())
-        o = ops().attn_decode_shared(q, cache.k, cache.v, prefix_table, prefix_lens, table, past, None, L, T, window, err())
+        q = cache.append(new[:, i: i + 1], table, past, None, *w, t_new[:, i: i + 1], f)
+        o = cache.attend(q, table, past, T, prefix_table, prefix_lens, L, window=window)
         past += 1
         end = L + i + 1
         yq, yk, yv = y[:, :end].double().view(S, end, 3, H, hd).unbind(2)
@@ -519,7 +518,8 @@ def test_c_abi_refuses_before_it_launches():
                 dict(ps=131072), dict(pt=None), dict(pl=None), dict(G=0), dict(G=4), dict(G=7), dict(tab=None), dict(past=None),
                 dict(o=None), dict(o=P + 2), dict(S=-1), dict(Lq=0), dict(Lq=17), dict(H=0), dict(hd=12), dict(hd=136), dict(hd=0),
                 dict(pcap=-1), dict(pcap=16385), dict(cap=0), dict(cap=129), dict(window=-1), dict(dt=2), dict(ws=None),
-                dict(ws=P + 4), dict(nb=64), dict(S=1 << 27)):
+                dict(ws=P + 4), dict(nb=64), dict(S=1 << 27), dict(S=1 << 22, H=16, hd=8), dict(tw=1 << 40),
+                dict(pw=1 << 31)):
         assert call(**bad) == 1, bad
     assert call(S=0) == 0
     need = lib.esgpt_attn_decode_shared_workspace
@@ -539,6 +539,8 @@ def test_fake_tensors():
 
 
 def test_paged_cache_hands_out_each_page_once():
+    from eventstreamgpt_amd import _lib as L
+    from eventstreamgpt_amd import kernels as K
     from eventstreamgpt_amd.kernels import PagedKV
 
     c = PagedKV(6, 16, 2, 32, torch.float32, "cpu")
@@ -551,6 +553,12 @@ def test_paged_cache_hands_out_each_page_once():
     assert sorted(c.pages(3).tolist() + b.tolist()) == list(range(6))
     with pytest.raises(ValueError, match="not handed out"):
         c.release(torch.tensor([0, 0]))
+    with pytest.raises(L.HipExtensionMissing):
+        c.append(torch.zeros(1, 1, 192), a[None, :1], a[:1])
+    with pytest.raises(NotImplementedError, match="no_grad"):
+        c.attend(torch.zeros(1, 1, 64, requires_grad=True), a[None, :1], a[:1], 16)
+    with pytest.raises(L.HipExtensionMissing):
+        K.qk_norm_rope(torch.zeros(1, 1, 192), None, None, None, None, 2)
     for ps in (8, 24, 1 << 17):
         with pytest.raises(ValueError, match="page size"):
             PagedKV(2, ps, 2, 32, torch.float32, "cpu")

@@ -395,13 +395,17 @@ def test_append_refusals():
         ({"k_pages": torch.zeros(1, H, 48, hd, device=DEV), "v_pages": torch.zeros(1, H, 48, hd, device=DEV)}, "page size"),
         ({"k_pages": kp[..., :8].contiguous(), "v_pages": vp[..., :8].contiguous()}, "heads of 8"),
         ({"page_table": table.long()}, "page_table"), ({"page_table": table[:1]}, "page_table"),
-        ({"page_table": table.t()}, "page_table"), ({"past": past.cpu()}, "past"), ({"past": past[:1]}, "past"),
+        ({"page_table": table.flatten()}, "page_table"), ({"past": past.cpu()}, "past"), ({"past": past[:1]}, "past"),
         ({"row_mask": torch.ones(2, 2, device=DEV).bool()}, "row_mask"), ({"row_mask": torch.ones(2, 3, device=DEV)}, "row_mask"),
         ({"err": torch.zeros(2, dtype=torch.int64)}, "error block"), ({"k_w": None}, "together"),
     ]:
         with pytest.raises(RuntimeError, match=text):
             ops().kv_append_paged(**{**ok, **change})
-    ops().kv_append_paged(**ok)
+    want = [t.clone() for t in (ops().kv_append_paged(**ok), kp, vp)]
+    wide = torch.full((2, 5), -1, device=DEV).int()  # a slice of a wider table
+    wide[:, 1:3] = table
+    got = ops().kv_append_paged(**{**ok, "page_table": wide[:, 1:3], "past": wide[:, 0] + 1})
+    assert all(torch.equal(a, b) for a, b in zip((got, kp, vp), want)) and int(err()[0]) == 0
 
 
 # ------------------------------------------------------------------------------------------- without a device
