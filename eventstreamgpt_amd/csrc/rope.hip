@@ -230,6 +230,13 @@ __global__ __launch_bounds__(kThreads, MODE == MODE_BWD ? 4 : 1) void rope_kerne
       }
       __syncthreads();
 
+      // the next token's loads, once this one's registers are free
+      auto ahead = [&](int t) {
+        const int u = t + a.slots;
+        if (u >= nt) return;
+        if (MODE == MODE_APPEND && dst[u] == kMasked) return;
+        fetch(n0 + u);
+      };
       for (int t = slot; t < nt; t += a.slots) {
         const int64_t n = n0 + t;
         int64_t d = 0;
@@ -241,10 +248,11 @@ __global__ __launch_bounds__(kThreads, MODE == MODE_BWD ? 4 : 1) void rope_kerne
               st<T, V>(out + n * D + col + lo, z);
               st<T, V>(out + n * D + col + hi, z);
             }
+            ahead(t);
             continue;
           }
         }
-        if (MODE == MODE_BWD || t != slot) fetch(n);
+        if (MODE == MODE_BWD) fetch(n);
         if (von) {
           if constexpr (MODE == MODE_APPEND) {
             if (d >= 0)
@@ -261,6 +269,7 @@ __global__ __launch_bounds__(kThreads, MODE == MODE_BWD ? 4 : 1) void rope_kerne
             fl[j] = on ? to_f32(xl.e[j]) : 0.f;
             fh[j] = on ? to_f32(xh.e[j]) : 0.f;
           }
+          if (MODE != MODE_BWD) ahead(t);
           float rstd = 1.f;
           if constexpr (NORM) {
             float ss = 0.f;
