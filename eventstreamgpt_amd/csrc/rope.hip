@@ -15,7 +15,11 @@
 // rotation partners (two 16-B accesses each way, so the rotation needs no exchange between lanes), the head's lanes
 // are neighbours in one wave (the norm's sum is a short DPP butterfly), and a thread keeps its (head, chunk) while it
 // walks tokens, so that weights stay in registers and the backward sums dw there. The sines and cosines of a token
-// are shared by its 2 H heads: the workgroup computes those of a run of tokens once, into LDS.
+// are shared by its 2 H heads: the workgroup computes those of a run of tokens once, into LDS, while the loads of its
+// first tokens are in flight; the next token's loads follow the current one's last use of the registers.
+// Measured (hd 64, bf16): 65,536 tokens of 8 heads forward 74 us (5.4 TB/s), backward 112 us + 4 of dw sum (4.8 TB/s; four
+// waves per SIMD, at three it was 167), a large copy's rate on this card being 4.95; 32 x 1024 rows appended, a third of
+// them padding, 4 heads 19 us (3.8 TB/s); 512 sequences' single rows 5.3 us, the chain of past, page id and store.
 #include "common.h"
 
 #include <algorithm>
@@ -412,9 +416,10 @@ struct Plan {
 };
 
 // V: the widest access (up to 16 B) that the rotated half and half of what is not rotated are whole multiples of.
-// The workgroup takes as many tokens at once as give it up to 256 lanes, and one to four such sets per run: more
-// tokens per run cost fewer barriers and workgroups (and fewer chains of loads to find a token's cache row), while
-// fewer keep the chip full (kRuns runs at least).
+// The workgroup takes as many tokens at once as give it up to 256 lanes (a set), and a few sets per run: more sets cost
+// fewer barriers, workgroups and (append) chains of loads to a token's cache row, fewer keep the chip full. Measured in
+// graph replays: forward of 65,536 x 512 at two / four sets a run 74.4 / 79.6 us; append of 32 x 1024 x 256 at one / two /
+// four / eight 33 / 21.1 / 19.1 / 22.1; backward of 8,192 x 256 in 512 / 1,024 workgroups 14.7 / 15.5 with its dw sum.
 Plan make_plan(int64_t N, int64_t H, int64_t hd, int64_t R, int dtype, int mode) {
   Plan p;
   const int64_t R2 = R / 2, tail = hd / 2 - R2;
@@ -429,8 +434,8 @@ Plan make_plan(int64_t N, int64_t H, int64_t hd, int64_t R, int dtype, int mode)
   p.passes = (int)cdiv(ipt, kThreads);
   p.slots = p.passes > 1 ? 1 : (int)std::min<int64_t>(kThreads / ipt, most / 2);
   p.block = p.passes > 1 ? kThreads : (int)(cdiv(p.slots * ipt, 64) * 64);
-  const int64_t kRuns = mode == MODE_FWD ? 2048 : 1024;
-  const int64_t sets = std::max<int64_t>(1, std::min<int64_t>({4, most / p.slots, N / (p.slots * kRuns)}));
+  const int64_t kRuns = mode == MODE_FWD ? 2048 : mode == MODE_BWD ? 512 : 1024, kSets = mode == MODE_APPEND ? 4 : 2;
+  const int64_t sets = std::max<int64_t>(1, std::min<int64_t>({kSets, most / p.slots, N / (p.slots * kRuns)}));
   p.run = (int)(p.slots * sets);
   p.grid = std::min<int64_t>(cdiv(N, p.run), mode == MODE_BWD ? 1024 : (int64_t)1 << 20);
   p.lds = 2 * hd * sizeof(float) + std::max<size_t>((size_t)p.run * R2, 8) * sizeof(float2);  // 8: see ct in the kernel
