@@ -54,7 +54,8 @@ struct SharedArgs {
   int32_t* err;
   int64_t n_pages, prefix_w, table_w;
   int S, n, Lq, H, hd, psl;     // psl: log2 of the page size
-  int prefix_cap, cap, window;  // window 0: none
+  int prefix_cap, cap;
+  int window, owin;             // the window where it can cut the history, the own rows (0: never)
   int M, RT;                    // rows of a group; row tiles of the history's workgroups
   int NPc, NSc, NP, pchunk, schunk;
   int units;  // history workgroups; the own rows' follow
@@ -654,17 +655,17 @@ __global__ __launch_bounds__(64 * kWaves, KD * NT < 8 ? 2 : 1) void shared_kerne
     OneSegment<1> sg;
     sg.tab = a.table + (int64_t)s * a.table_w;
     sg.step = W::KB;
-    sg.raw = a.window ? -1 : x.pages(sg.tab, ch * a.schunk, W::KB, a.cap);
+    sg.raw = a.owin ? -1 : x.pages(sg.tab, ch * a.schunk, W::KB, a.cap);
     typename W::Q q[1];
     x.load_q(q[0], (int64_t)s * a.Lq + c, c < a.Lq);
     const Row r = row_of(a, s, c, c < a.Lq);
     sg.act[0] = r.active;
     sg.hi[0] = r.active ? min(r.at + 1, a.cap) : 0;
-    sg.lo[0] = (r.active && a.window) ? max(0, r.at - a.window + 1) : 0;
+    sg.lo[0] = (r.active && a.owin) ? max(0, r.at - a.owin + 1) : 0;
     const int base = cols_min(r.active ? sg.lo[0] : a.cap) & ~15, end = cols_max(sg.hi[0]);  // no active row: no key
     sg.first = base + ch * a.schunk;
     sg.end = min(end, sg.first + a.schunk);
-    if (a.window && sg.first < sg.end) sg.raw = x.pages(sg.tab, sg.first, W::KB, sg.end);
+    if (a.owin && sg.first < sg.end) sg.raw = x.pages(sg.tab, sg.first, W::KB, sg.end);
     State<1, W::DT> st;
     x.walk(st, q, sg);
     const float l = r.active ? xsum(st.l[0]) : 0.f;
@@ -756,11 +757,10 @@ __global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
         k0 = cols_min(mine ? olo : a.cap) & ~15;
         k_end = cols_max(mine ? ohi : 0);
       }
-      if (a.window) {
+      if (seg == 0 ? a.window : a.owin) {
         if (k0 < k_end) raw = x.pages(table(seg), k0, stride(seg), k_end);
-      } else if (seg + 1 < count) {
-        ids = x.pages(table(seg + 1), 0, W::KB, a.cap);
       }
+      if (!a.owin && seg + 1 < count) ids = x.pages(table(seg + 1), 0, W::KB, a.cap);
     }
     __device__ __forceinline__ void limits(int seg, int (&lo)[1], int (&hi)[1], int& lo_all, int& hi_all) const {
       if (seg == 0) {
@@ -787,11 +787,10 @@ __global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
   sg.my = grp * a.n + rr / a.Lq;  // this column's trajectory
   const Row r = row_of(a, sg.my, rr % a.Lq, rr < a.M);
   sg.act = r.active;
-  const bool cut = r.active && a.window;
   sg.phi = r.active ? sg.P : 0;
-  sg.plo = cut ? min(sg.P, max(0, sg.P + r.at - a.window + 1)) : 0;
+  sg.plo = (r.active && a.window) ? min(sg.P, max(0, sg.P + r.at - a.window + 1)) : 0;
   sg.ohi = r.active ? min(r.at + 1, a.cap) : 0;
-  sg.olo = cut ? max(0, r.at - a.window + 1) : 0;
+  sg.olo = (r.active && a.owin) ? max(0, r.at - a.owin + 1) : 0;
   State<1, W::DT> st;
   x.walk(st, q, sg);
   J::run(a, st, 0, r.active, lds, out0, rt * 16, h, 0);
@@ -933,6 +932,9 @@ int launch_shared(const SharedPlan& p, const SharedArgs& a, hipStream_t st) {
   return ESGPT_OK;
 }
 
+// 0 for a window that no distance within the caps leaves.
+int64_t cut_window(int64_t window, int64_t prefix_cap, int64_t cap) { return window < prefix_cap + cap ? window : 0; }
+
 bool shared_ok(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap, int64_t cap, int64_t window,
                int dtype) {
   return G > 0 && S >= G && S % G == 0 && Lq >= 1 && Lq <= kMaxLq && H > 0 && hd > 0 && hd <= 128 &&
@@ -948,7 +950,7 @@ extern "C" {
 size_t esgpt_attn_decode_shared_workspace(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap,
                                           int64_t cap, int64_t window, int dtype) {
   if (!shared_ok(G, S, Lq, H, hd, prefix_cap, cap, window, dtype)) return 0;
-  const SharedPlan p = shared_plan(G, S, Lq, H, hd, prefix_cap, cap, std::min<int64_t>(window, (int64_t)1 << 30), dtype);
+  const SharedPlan p = shared_plan(G, S, Lq, H, hd, prefix_cap, cap, cut_window(window, prefix_cap, cap), dtype);
   return p.NP > 1 ? (size_t)(S * Lq * H * p.NP) * (2 + hd) * sizeof(float) : 0;
 }
 
@@ -966,7 +968,7 @@ int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_p
   auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
   ESGPT_REQUIRE(q && o && past && page_table && aligned(q) && aligned(o) && (prefix_cap == 0 || (prefix_table && prefix_lens)));
   ESGPT_REQUIRE(n_pages == 0 || (k_pages && v_pages && aligned(k_pages) && aligned(v_pages)));
-  window = std::min<int64_t>(window, (int64_t)1 << 30);
+  window = cut_window(window, prefix_cap, cap);
   const SharedPlan p = shared_plan(G, S, Lq, H, hd, prefix_cap, cap, window, dtype);
   // a launch holds fewer than 2^32 threads
   constexpr int64_t kThreads = ((int64_t)1 << 32) - 1;
@@ -1002,6 +1004,7 @@ int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_p
   a.prefix_cap = (int)prefix_cap;
   a.cap = (int)cap;
   a.window = (int)window;
+  a.owin = window < cap ? (int)window : 0;
   a.M = (int)((S / G) * Lq);
   a.RT = p.RT;
   a.NPc = p.NPc;
