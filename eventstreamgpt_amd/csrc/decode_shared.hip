@@ -13,7 +13,7 @@
 // nothing as long as memory is the bound (a bf16 tile of 16 keys x 64 takes 64 MFMA cycles for 4 KB, 64 B per cycle and
 // SIMD, against the 13 B per cycle that HBM gives a whole CU).
 //
-// Two forms (shared_plan chooses and holds the measurements). Whole: one workgroup per (group, head, 16 rows) does the
+// Two forms (shared_plan chooses and holds the measurements). Whole: one workgroup per (group, head, 4..16 rows) does the
 // history and the own rows and writes the result. Split: the history of each (group, head, 16 or 32 rows) is cut into
 // chunks, one workgroup each, whose four waves take every fourth block of keys and join through LDS, and the own rows of
 // each (trajectory, head) into chunks of one wave; each part leaves (m, l, O) in f32 and a second kernel joins a row's
@@ -56,7 +56,7 @@ struct SharedArgs {
   int S, n, Lq, H, hd, psl;     // psl: log2 of the page size
   int prefix_cap, cap;
   int window, owin;             // the window where it can cut the history, the own rows (0: never)
-  int M, RT;                    // rows of a group; row tiles of the history's workgroups
+  int M, RT, tr;                // rows of a group; row tiles of the history's workgroups; whole form: rows of a tile
   int NPc, NSc, NP, pchunk, schunk;
   int units;  // history workgroups; the own rows' follow
 };
@@ -539,21 +539,21 @@ __device__ __forceinline__ void emit4(const SharedArgs& a, int64_t out, int h, i
 }
 
 // The waves' states of one tile of 16 rows, joined per row through LDS, 64 dimensions at a time: row r0 + i of the group
-// is column i. Every thread of the workgroup calls this.
+// is column i < n. Every thread of the workgroup calls this.
 template <typename T, int KD, int NW>
 struct Join {
   static constexpr int W = KD * 32 < 64 ? KD * 32 : 64, OLD = W + 4;
   static constexpr int kBytes = NW * 16 * (OLD + 2) * 4;
   template <int NT>
   __device__ __forceinline__ static void run(const SharedArgs& a, const State<NT, 2 * KD>& st, int t, bool act, char* lds,
-                                             int64_t out0, int r0, int h, int part) {
+                                             int64_t out0, int r0, int n, int h, int part) {
     const int w = scalar(threadIdx.x >> 6), lane = lane_id(), g = lane >> 4, c = lane & 15;
     float* jo = reinterpret_cast<float*>(lds);  // [wave][16][OLD]
     float* jm = jo + NW * 16 * OLD;             // [wave][16]
     float* jl = jm + NW * 16;
     const float lw = act ? xsum(st.l[t]) : 0.f;
     const int row = threadIdx.x >> 4;
-    const bool mine = row < 16 && r0 + row < a.M;
+    const bool mine = row < n && r0 + row < a.M;
     float M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int d0 = 0; d0 < KD * 32; d0 += W) {
@@ -717,11 +717,11 @@ __global__ __launch_bounds__(64 * kWaves, KD * NT < 8 ? 2 : 1) void shared_kerne
   }
   State<NT, W::DT> st;
   x.walk(st, q, sg);
-  J::run(a, st, 0, sg.act[0], lds, out0, rt * 16 * NT, h, ch);
-  if constexpr (NT == 2) J::run(a, st, 1, sg.act[1], lds, out0, rt * 16 * NT + 16, h, ch);
+  J::run(a, st, 0, sg.act[0], lds, out0, rt * 16 * NT, 16, h, ch);
+  if constexpr (NT == 2) J::run(a, st, 1, sg.act[1], lds, out0, rt * 16 * NT + 16, 16, h, ch);
 }
 
-// Whole form: one workgroup of NW waves per (group, head, 16 rows) does the rows' history and their own rows and writes
+// Whole form: one workgroup of NW waves per (group, head, `tr` rows) does the rows' history and their own rows and writes
 // the result. The waves take every NW-th block of the history (segment 0) and, from the other end, every NW-th
 // trajectory's own rows, which only that trajectory's columns see; a segment's page ids are loaded when the one before is
 // opened.
@@ -777,15 +777,16 @@ __global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
     }
   };
 
-  const int rr = rt * 16 + c, s0 = grp * a.n + rt * 16 / a.Lq;
-  const int ns = grp * a.n + min(a.M - 1, rt * 16 + 15) / a.Lq - s0 + 1;
+  const int rr = rt * a.tr + c, s0 = grp * a.n + rt * a.tr / a.Lq;
+  const int ns = grp * a.n + min(a.M, rt * a.tr + a.tr) / a.Lq - s0 + (min(a.M, rt * a.tr + a.tr) % a.Lq != 0);
+  const bool exists = c < a.tr && rr < a.M;
   Segs sg{a, a.prefix_table + (int64_t)grp * a.prefix_w, w, s0, 1 + max(0, (ns - (NW - 1 - w) + NW - 1) / NW)};
   sg.ids = a.window ? -1 : x.pages(sg.ptab, w * W::KB, sg.stride(0), a.prefix_cap);
   typename W::Q q[1];
-  x.load_q(q[0], out0 + rr, rr < a.M);
+  x.load_q(q[0], out0 + rr, exists);
   sg.P = prefix_len(a, grp);
   sg.my = grp * a.n + rr / a.Lq;  // this column's trajectory
-  const Row r = row_of(a, sg.my, rr % a.Lq, rr < a.M);
+  const Row r = row_of(a, sg.my, rr % a.Lq, exists);
   sg.act = r.active;
   sg.phi = r.active ? sg.P : 0;
   sg.plo = (r.active && a.window) ? min(sg.P, max(0, sg.P + r.at - a.window + 1)) : 0;
@@ -793,7 +794,7 @@ __global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
   sg.olo = (r.active && a.owin) ? max(0, r.at - a.owin + 1) : 0;
   State<1, W::DT> st;
   x.walk(st, q, sg);
-  J::run(a, st, 0, r.active, lds, out0, rt * 16, h, 0);
+  J::run(a, st, 0, r.active, lds, out0, rt * a.tr, a.tr, h, 0);
 }
 
 // Joins a row's parts: o = sum_p e^{m_p - M} O_p / sum_p e^{m_p - M} l_p. One wave per (row, head): lane groups of
@@ -833,7 +834,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a, int64_t 
 }
 
 struct SharedPlan {
-  int whole, NT, RT, NPc, NSc, NP, pchunk, schunk;
+  int whole, tr, NT, RT, NPc, NSc, NP, pchunk, schunk;
   int64_t units, own_blocks;
 };
 
@@ -845,18 +846,21 @@ int block_keys(int64_t hd, int dtype) {
                              : (hd <= 64 ? Walk<float, 2>::KB : Walk<float, 4>::KB);
 }
 
-// Whole or split. The whole form saves the second launch and the parts' traffic but has 16 rows' keys on one CU; what it
-// costs is its busiest wave's chain of blocks (steps: those of the history and those of its trajectories' own rows).
-// Measured in graph replays, whole / split us (groups x trajectories, history + own rows, heads, head size):
-//   every block and trajectory has a wave of its own: 8x4 100+10 h4 hd64 bf16 6.7 / 7.9; 1x4 40+6 f32 hd16 6.3 / 7.1
-//     (not so: 4x8 200+20 f32 8.6 / 7.6)
-//   half the CUs or more have a workgroup, three steps: 32x16 256+64 h4 13.1 / 14.8 (64 workgroups, 16x4 1024+32: 12.8 / 11.5)
-//   one workgroup per CU or more: 32x8 512+24 window 32 9.2 / 14.4; 64x4 300+20 11.3 / 12.4; 32x16 2048+32 h8 35.5 / 39.3;
-//     unless the own rows are the longer chain: 64x1 512+400 34.9 / 24.9.
+// Whole or split. The whole form saves the second launch and the parts' traffic but has a tile's keys on one CU; what it
+// costs is its busiest wave's chain of blocks (steps: those of the history and those of its trajectories' own rows). A tile
+// is 16 rows, or 8 or 4 while there are fewer workgroups than CUs: the history is then read by more of them, out of L2, and
+// each has fewer trajectories (32x16 256+64: 16 rows 12.9, 8 rows 11.4).
+// Measured in graph replays, whole / split us (groups x trajectories, history + own rows, heads; hd 64 bf16 if not said):
+//   every block and trajectory has a wave of its own: 8x4 100+10 h4 6.8 / 7.9; 1x4 40+6 h4 f32 hd16 6.3 / 7.2
+//     (not so: 4x8 200+20 h4 f32 hd16 8.1 / 7.7)
+//   16-row tiles for every CU: 32x8 512+24 window 32 h8 8.3 / 14.3; 64x4 300+20 h4 11.0 / 12.2; 32x16 2048+32 h8 35.4 / 39.5;
+//     unless the own rows are the longer chain: 64x1 512+400 h8 34.9 / 24.9
+//   smaller tiles for half the CUs or more, and a chain of at most three: 32x16 256+64 h4 11.4 / 15.0; 32x8 256+64 h4 9.1 /
+//     11.5; 16x16 256+64 h4 f32 14.1 / 14.9 (a longer history: 4x16 1000+20 h8 12.3 / 9.9, 4x64 2048+32 h8 18.8 / 16.7)
 // Without a history the split form's waves are the whole of it, and write directly where one chunk holds a trajectory.
-// The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 55.8 / 58.8, 8x8 8192+32 f32 50.7 /
-// 52.2, 16x4 1024+33 f32 15.0 / 18.2, 4x64 2048+32 16.9 / 20.1 (more parts cost more joins); own rows at 1,024 waves: 16x16
-// 256+64 f32 15.7 against 19.7 at 4,096.
+// The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 55.8 / 58.8, 8x8 8192+32 h8 f32 50.7 /
+// 52.2, 16x4 1024+33 h4 f32 15.0 / 18.2, 4x64 2048+32 h8 16.9 / 20.1 (more parts cost more joins); own rows at 1,024 waves:
+// 16x16 256+64 f32 15.7 against 19.7 at 4,096.
 SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap, int64_t cap,
                        int64_t window, int dtype) {
   SharedPlan p;
@@ -864,13 +868,15 @@ SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, 
   const int64_t M = (S / G) * Lq, kb = block_keys(hd, dtype), nw = whole_waves(hd);
   const int64_t pspan = window ? std::min(prefix_cap, window + 16) : prefix_cap;
   const int64_t sspan = window ? std::min(cap, window + Lq + 16) : cap;
-  const int64_t seqs = std::min<int64_t>(cdiv(std::min<int64_t>(M, 16), Lq) + (Lq > 1), S / G);  // of 16 rows
+  p.tr = 16;
+  while (p.tr > 4 && G * H * cdiv(M, p.tr) < kCus) p.tr /= 2;
+  const int64_t seqs = std::min<int64_t>(cdiv(std::min<int64_t>(M, p.tr), Lq) + (Lq > 1), S / G);  // of a tile
   const int64_t steps = cdiv(pspan, nw * kb), own_steps = cdiv(seqs, nw) * cdiv(sspan, kb);
-  p.RT = (int)cdiv(M, 16);
+  p.RT = (int)cdiv(M, p.tr);
   p.units = G * H * p.RT;
-  p.whole = pspan > 0 &&
-            (cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw || (p.units >= kCus / 2 && steps + own_steps <= 3) ||
-             (p.units >= kCus && own_steps <= std::max<int64_t>(4, steps)));
+  p.whole = pspan > 0 && (cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw ||
+                          (p.tr == 16 && p.units >= kCus && own_steps <= std::max<int64_t>(4, steps)) ||
+                          (p.units >= kCus / 2 && steps <= 1 && own_steps <= 2));
   if (p.whole) {
     p.NT = p.NP = 1;
     p.NPc = p.NSc = p.pchunk = p.schunk = 0;
@@ -1007,6 +1013,7 @@ int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_p
   a.owin = window < cap ? (int)window : 0;
   a.M = (int)((S / G) * Lq);
   a.RT = p.RT;
+  a.tr = p.tr;
   a.NPc = p.NPc;
   a.NSc = p.NSc;
   a.NP = p.NP;
