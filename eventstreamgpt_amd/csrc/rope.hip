@@ -555,8 +555,9 @@ int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, c
                           const int32_t* page_table, int64_t table_w, void* k_pages, void* v_pages, int64_t n_pages,
                           int64_t page_size, void* q, int64_t S, int64_t Lq, int64_t H, int64_t hd, int dtype,
                           int32_t* err, void* stream) {
-  constexpr int64_t kTop = ((int64_t)1 << 31) - 1024;  // the kernel counts tokens in 32 bits
-  ESGPT_REQUIRE(S >= 0 && Lq >= 0 && Lq <= kTop && S <= kTop && S * Lq <= kTop);
+  // the kernel counts tokens in 32 bits, and a sequence's kept rows in f32
+  constexpr int64_t kTop = ((int64_t)1 << 31) - 1024;
+  ESGPT_REQUIRE(S >= 0 && Lq >= 0 && Lq <= (int64_t)1 << 24 && S <= kTop && S * Lq <= kTop);
   ESGPT_REQUIRE(rope_ok(qkv, q_w, k_w, pos, pos_dtype, inv_freq, R, S * Lq, H, hd, eps, dtype));
   ESGPT_REQUIRE(page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0 && table_w >= 0 &&
                 table_w < (int64_t)1 << 31 && n_pages >= 0 && n_pages < (int64_t)1 << 31);

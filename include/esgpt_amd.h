@@ -242,9 +242,9 @@ int esgpt_attn_decode(const void* q, int64_t ld_q, const void* k_cache, const vo
  *   cache. k_pages / v_pages: [n_pages, H, page_size, hd] (a head's rows of one page are contiguous; page_size a
  *   power of two, 16..65536); page_table int32 [S, table_w]. Row i of sequence s goes to cache row past[s] + (rows
  *   before i that row_mask [S, Lq] keeps; NULL: all), i.e. padded rows are not stored; q [S, Lq, D] gets the
- *   normalised, rotated queries (zeros in padded rows). A row beyond the table, a negative past or a page outside
- *   [0, n_pages) raises ESGPT_FLAG_BAD_PAGE and is not stored. Cache rows must be distinct: two sequences that name
- *   the same page and write the same row of it leave either's values there. */
+ *   normalised, rotated queries (zeros in padded rows). Lq <= 2^24, S * Lq <= 2^31 - 1024. A row beyond the table, a
+ *   negative past or a page outside [0, n_pages) raises ESGPT_FLAG_BAD_PAGE and is not stored. Cache rows must be
+ *   distinct: two sequences that name the same page and write the same row of it leave either's values there. */
 int esgpt_qk_norm_rope_fwd(const void* qkv, const float* q_w, const float* k_w, const void* pos, int pos_dtype,
                            const float* inv_freq, int64_t R, int64_t N, int64_t H, int64_t hd, float eps, void* out,
                            int dtype, void* stream);

@@ -448,7 +448,8 @@ def test_c_abi_refuses_before_it_launches():
                                          64, 1, None, None)
 
     for bad in (dict(past=None), dict(tab=None), dict(W=-1), dict(kp=None), dict(kp=P + 4), dict(n_pages=-1), dict(ps=8),
-                dict(ps=48), dict(ps=131072), dict(q=None), dict(S=-1), dict(Lq=-1)):
+                dict(ps=48), dict(ps=131072), dict(q=None), dict(S=-1), dict(Lq=-1), dict(S=1, Lq=(1 << 24) + 1),
+                dict(S=1 << 20, Lq=1 << 11), dict(W=1 << 31)):
         assert app(**bad) == 1, bad
     assert app(S=0) == 0 and app(Lq=0) == 0
 
