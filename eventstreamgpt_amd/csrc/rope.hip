@@ -375,6 +375,7 @@ __global__ __launch_bounds__(kThreads, MODE == MODE_BWD ? 4 : 1) void rope_kerne
         float* p = a.part + (int64_t)blockIdx.x * 2 * hd + o;
         *p = pass > 0 ? *p + sum : sum;  // the same thread every pass
       }
+      __syncthreads();  // the next pass writes the weights over buf
     }
   }
 }

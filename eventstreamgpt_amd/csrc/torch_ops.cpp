@@ -720,8 +720,8 @@ Tensor attn_decode_shared(const Tensor& q_, const Tensor& k_pages, const Tensor&
   const size_t nb = esgpt_attn_decode_shared_workspace(G, S, Lq, H, hd, prefix_cap, cap, window, dt);
   Tensor ws = at::empty({(int64_t)nb}, q.options().dtype(at::kByte));
   check(esgpt_attn_decode_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.size(0), ps,
-                                 ptr<const int32_t>(ptab), pre ? ptab.size(1) : 0, ptr<const int32_t>(plen), G, ptr<const int32_t>(page_table),
-                                 page_table.size(1), ptr<const int32_t>(past),
+                                 ptr<const int32_t>(ptab), pre ? ptab.size(1) : 0, ptr<const int32_t>(plen), G,
+                                 ptr<const int32_t>(page_table), page_table.size(1), ptr<const int32_t>(past),
                                  m.defined() ? ptr<const uint8_t>(m) : nullptr, o.data_ptr(), S, Lq, H, hd, prefix_cap,
                                  cap, window, dt, ws.data_ptr(), nb, e, stream_of(q)),
         "attn_decode_shared");

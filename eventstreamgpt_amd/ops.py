@@ -32,11 +32,11 @@ Used by the NA glue's autograd Functions (transformer/structured_attention.py): 
 ``na_assemble`` / ``na_assemble_bwd`` (structured_attention.py:63-156).
 
 Non-differentiable: ``embed_bag_bwd``, ``embed_epilogue_bwd``, ``attention_bwd``, ``residual_ln_bwd``,
-``bias_act_bwd``, ``qk_norm_rope_bwd``, ``linear_act``, ``linear_bwd`` (+ ``weight_grad_join``: with ``dw_tickets`` the weight gradient
-runs on a second stream, joined by that op), ``gemm`` / ``gemm_``, ``column_sum``, ``kv_append``,
-``attn_decode`` (generation), ``kv_append_paged`` (the same norm and rotation into a paged cache),
-``attn_decode_shared`` (attention over it, a history shared by several trajectories read once), ``pack`` (the compute-dtype parameter copies) and ``adamw``
-(generative_modeling.py:460-485).
+``bias_act_bwd``, ``qk_norm_rope_bwd``, ``linear_act``, ``linear_bwd`` (+ ``weight_grad_join``: with ``dw_tickets``
+the weight gradient runs on a second stream, joined by that op), ``gemm`` / ``gemm_``, ``column_sum``, ``kv_append``,
+``attn_decode`` (generation), ``kv_append_paged`` (``qk_norm_rope`` on the way into a paged cache),
+``attn_decode_shared`` (attention over it, a history shared by several trajectories read once), ``pack`` (the
+compute-dtype parameter copies) and ``adamw`` (generative_modeling.py:460-485).
 
 There is no CPU kernel: calling an operator on CPU tensors raises (no fallback).
 """

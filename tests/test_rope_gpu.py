@@ -74,6 +74,8 @@ SHAPES = [
     (1, 1, 4, 64, 64), (4, 16, 4, 16, 16), (2, 33, 1, 8, 8), (3, 7, 5, 24, 8), (2, 9, 3, 24, 12), (2, 5, 2, 40, 6),
     (1, 3, 2, 128, 2), (2, 70, 8, 64, 32), (1, 17, 12, 96, 96), (1, 5, 9, 128, 2), (1, 4, 40, 128, 128),
     (33, 129, 4, 64, 64), (2, 31, 4, 64, 0),
+    # three and eight passes of a workgroup over one token's lanes, whose dw sums share memory with the next pass's weights
+    (3, 41, 80, 128, 64), (1, 700, 128, 128, 128),
 ]
 
 
@@ -330,6 +332,7 @@ def append_oracle(y, kp, vp, table, past, mask, H):
 @pytest.mark.parametrize("S,Lq,H,hd,R,ps,masked", [
     (1, 1, 1, 8, 8, 16, False), (5, 1, 4, 64, 64, 64, False), (3, 40, 4, 16, 16, 16, True), (4, 77, 2, 24, 12, 32, True),
     (2, 300, 4, 64, 64, 128, True), (3, 5, 9, 128, 2, 16, True), (6, 3, 2, 32, 0, 16, False),
+    (3, 21, 80, 128, 64, 16, True),
 ], ids=str)
 def test_append(S, Lq, H, hd, R, ps, masked, dt):
     """Ragged pasts, left, right and scattered padding, pages in any order; every other row of the pools as it was."""
