@@ -690,7 +690,7 @@ class PagedKV:
         return torch.tensor([self._free.pop() for _ in range(count)], dtype=torch.int32, device=self.k.device)
 
     def release(self, ids: torch.Tensor) -> None:
-        ids = [int(i) for i in ids.tolist()]
+        ids = ids.flatten().tolist()
         if len(set(ids)) != len(ids) or not all(0 <= i < self.k.shape[0] for i in ids) or set(ids) & set(self._free):
             raise ValueError(f"pages {ids} are not handed out (each once)")
         self._free.extend(ids)
