@@ -565,7 +565,8 @@ std::tuple<Tensor, Tensor> qk_norm_rope_bwd(const Tensor& dout_, const Tensor& q
   const RopeIn r = rope_in("esgpt.qk_norm_rope_bwd", qkv_, qkv_.size(0), qkv_.size(1), hd, q_w, k_w, pos, inv_freq);
   TORCH_CHECK(dout_.sizes() == qkv_.sizes() && dout_.device() == qkv_.device(),
               "esgpt.qk_norm_rope_bwd: dout must have the shape and device of qkv");
-  Tensor qkv = rows16(qkv_), dout = rows16(dout_.to(qkv_.scalar_type()));
+  Tensor qkv = rows16(qkv_);
+  Tensor dout = rows16(dout_.scalar_type() == qkv_.scalar_type() ? dout_ : dout_.to(qkv_.scalar_type()));
   const int64_t N = qkv.size(0) * qkv.size(1);
   const int dt = dtype_code(qkv.scalar_type());
   Tensor dqkv = at::empty(qkv.sizes(), qkv.options());
@@ -603,6 +604,8 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("esgpt::qk_norm_rope_bwd", "")
                          .typed<decltype(qk_norm_rope_bwd)>();
+    optional<at::AutoDispatchBelowADInplaceOrView> guard;  // unless this backward is itself recorded: straight to the kernel
+    if (!at::GradMode::is_enabled()) guard.emplace();
     auto s = ctx->get_saved_variables();
     auto o = [](const Tensor& x) { return x.defined() ? optional<Tensor>(x) : optional<Tensor>(); };
     auto [dqkv, dw] = op.call(grads[0], s[0], o(s[1]), o(s[2]), o(s[3]), o(s[4]), ctx->saved_data["H"].toInt(),
