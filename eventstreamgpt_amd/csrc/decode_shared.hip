@@ -854,13 +854,18 @@ int block_keys(int64_t hd, int dtype) {
 //   every block and trajectory has a wave of its own: 8x4 100+10 h4 6.8 / 7.9; 1x4 40+6 h4 f32 hd16 6.3 / 7.2
 //     (not so: 4x8 200+20 h4 f32 hd16 8.1 / 7.7)
 //   16-row tiles for every CU: 32x8 512+24 window 32 h8 8.3 / 14.3; 64x4 300+20 h4 11.0 / 12.2; 32x16 2048+32 h8 35.4 / 39.5;
-//     unless the own rows are the longer chain: 64x1 512+400 h8 34.9 / 24.9
+//     unless few trajectories' own rows make one wave's chain far longer than the others': 64x1 512+400 h8 34.9 / 24.9, 64x2
+//     39.3 / 34.8; even among the waves: 32x16 512+300 h8 55.6 / 59.2, 32x16 512+128 h8 f32 55.0 / 64.7
 //   smaller tiles for half the CUs or more, and a chain of at most three: 32x16 256+64 h4 11.4 / 15.0; 32x8 256+64 h4 9.1 /
 //     11.5; 16x16 256+64 h4 f32 14.1 / 14.9 (a longer history: 4x16 1000+20 h8 12.3 / 9.9, 4x64 2048+32 h8 18.8 / 16.7)
 // Without a history the split form's waves are the whole of it, and write directly where one chunk holds a trajectory.
 // The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 55.8 / 58.8, 8x8 8192+32 h8 f32 50.7 /
 // 52.2, 16x4 1024+33 h4 f32 15.0 / 18.2, 4x64 2048+32 h8 16.9 / 20.1 (more parts cost more joins); own rows at 1,024 waves:
-// 16x16 256+64 f32 15.7 against 19.7 at 4,096.
+// 16x16 256+64 f32 15.7 against 19.7 at 4,096. In f32 up to 32 dimensions a workgroup has little in flight, and two a CU pay:
+// 8x32 8192+32 h8 hd32 55.1 -> 42.2, 2x64 4096+32 h8 hd16 16.9 -> 15.0 (bf16 19.3 -> 20.6, 10.7 -> 10.6).
+// History tiles of 32 rows halve the reads and, in f32, the chunks left to a wave pay for the second accumulator only where
+// there are many: 16 / 32 rows 4x32 16384+32 h8 78.6 / 66.1, 16x32 4096+32 83.4 / 71.4, 32x32 2048 90.2 / 82.5; 8x32 2048 27.8 /
+// 28.4, 2x64 4096 h4 19.0 / 21.0 (and above 64 dimensions its registers spill).
 SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap, int64_t cap,
                        int64_t window, int dtype) {
   SharedPlan p;
@@ -872,10 +877,11 @@ SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, 
   while (p.tr > 4 && G * H * cdiv(M, p.tr) < kCus) p.tr /= 2;
   const int64_t seqs = std::min<int64_t>(cdiv(std::min<int64_t>(M, p.tr), Lq) + (Lq > 1), S / G);  // of a tile
   const int64_t steps = cdiv(pspan, nw * kb), own_steps = cdiv(seqs, nw) * cdiv(sspan, kb);
+  const bool even = 2 * nw * (steps + own_steps) <= 3 * (cdiv(pspan, kb) + seqs * cdiv(sspan, kb));
   p.RT = (int)cdiv(M, p.tr);
   p.units = G * H * p.RT;
   p.whole = pspan > 0 && (cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw ||
-                          (p.tr == 16 && p.units >= kCus && own_steps <= std::max<int64_t>(4, steps)) ||
+                          (p.tr == 16 && p.units >= kCus && (own_steps <= std::max<int64_t>(4, steps) || even)) ||
                           (p.units >= kCus / 2 && steps <= 1 && own_steps <= 2));
   if (p.whole) {
     p.NT = p.NP = 1;
@@ -883,11 +889,12 @@ SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, 
     p.own_blocks = 0;
     return p;
   }
-  p.NT = dtype == ESGPT_BF16 && M > 16 ? 2 : 1;
+  const int64_t round = kWaves * kb, want = dtype == ESGPT_F32 && hd <= 32 ? 2 * kCus : kCus;
+  const bool many = G * H * cdiv(M, 32) * pspan >= 8 * want * round;  // eight blocks a wave
+  p.NT = M > 16 && (dtype == ESGPT_BF16 || (hd <= 64 && many)) ? 2 : 1;
   p.RT = (int)cdiv(M, 16 * p.NT);
-  const int64_t round = kWaves * kb;
   const int64_t base = G * H * p.RT;
-  p.NPc = pspan ? (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(kCus, base), cdiv(pspan, round), 48})) : 0;
+  p.NPc = pspan ? (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(want, base), cdiv(pspan, round), 48})) : 0;
   p.pchunk = p.NPc ? (int)(cdiv(cdiv(pspan, p.NPc), round) * round) : 0;
   p.NPc = p.NPc ? (int)cdiv(pspan, p.pchunk) : 0;
   p.NSc = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(4 * kCus, S * H), cdiv(sspan, 2 * kb), 16}));
@@ -914,7 +921,7 @@ int launch_shared(const SharedPlan& p, const SharedArgs& a, hipStream_t st) {
   }
 #define SHARED(KD)                                                                        \
   do {                                                                                    \
-    if constexpr (sizeof(T) == 2) {                                                       \
+    if constexpr (sizeof(T) == 2 || KD <= 2) {                                            \
       if (p.NT == 2) {                                                                    \
         shared_kernel<T, KD, 2><<<grid, block, 0, st>>>(a);                               \
         break;                                                                            \

@@ -143,6 +143,7 @@ CASES = [
     # enough (group, head)s for one workgroup each to do history and own rows in one launch
     (16, 9, 1, 8, 64, 32, 100, 40, 0), (32, 3, 2, 4, 128, 16, 70, 20, 0), (16, 3, 1, 8, 96, 16, 90, 12, 20),
     (33, 2, 1, 8, 40, 16, 20, 5, 0), (32, 20, 1, 4, 24, 16, 33, 9, 0), (32, 2, 5, 8, 16, 16, 600, 70, 0),
+    (64, 8, 1, 4, 16, 16, 30, 200, 0), (64, 8, 1, 4, 64, 16, 60, 200, 150),  # own rows are most of it, even among the waves
     (64, 1, 1, 4, 64, 64, 20, 400, 0), (1, 100, 1, 1, 64, 64, 90, 12, 0), (70, 1, 1, 4, 64, 16, 0, 90, 0),
 ]
 
@@ -306,6 +307,41 @@ def test_bounds_wider_than_the_lengths():
         x.check(x.run(), want)
         x.P, x.s = 400, 300
         x.check(x.run(prefix_cap=x.prefix_table.shape[1] * 16, cap=x.table.shape[1] * 16), want)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", [(2, 33, 1, 8, 64, 16, 300, 20, 0), (2, 25, 2, 8, 20, 64, 700, 20, 0), (1, 70, 1, 16, 32, 16, 90, 9, 0)],
+                         ids=str)
+def test_tiles_of_32_rows_over_long_bounds(c, dt):
+    """Bounds that a long history would need (the work is split by them) over short ones: f32 takes 32 rows a tile too."""
+    x = Case(*c, dt=dt) if c[4] % 8 == 0 or dt == F32 else Case(*c[:4], 24, *c[5:], dt=dt)
+    want = x.oracle()
+    x.prefix_table = torch.cat([x.prefix_table, torch.full((x.G, 16384 // x.ps), -1).int()], 1)
+    cap = x.prefix_table.shape[1] * x.ps
+    got = x.run(prefix_cap=cap)
+    x.P = cap
+    x.check(got, want)
+    assert int(err()[0]) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+def test_long_windows_and_an_infinity_at_their_edges(dt):
+    """32 rows a tile whose windows of 8,500 begin at different history rows; then an infinity where some begin."""
+    x = Case(2, 20, 1, 16, 40, 64, 9000, 30, 8500, dt=dt, seed=5)
+    x.prefix_lens = torch.tensor([9000, 8777]).int()
+    want = x.oracle()
+    got = x.run()
+    x.check(got, want)
+    j = 9000 - 8500 + 12  # seen by the first group's rows with at most 11 own rows before them
+    x.vp[x.prefix_table[0, j // 64], 3, j % 64, 7] = math.inf
+    sees = torch.zeros(x.S, 1, x.H, x.hd, dtype=torch.bool)
+    sees[:20, 0, 3, 7] = 9000 + x.past[:20] - j < 8500
+    assert sees.any() and not sees[:20, 0, 3, 7].all()
+    dirty = x.run().view(sees.shape)
+    assert not torch.isfinite(dirty.cpu()[sees]).any()
+    x.check(torch.where(sees.to(DEV), got.view(sees.shape), dirty), want)
 
 
 @gpu
