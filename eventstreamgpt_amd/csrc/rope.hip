@@ -17,9 +17,9 @@
 // walks tokens, so that weights stay in registers and the backward sums dw there. The sines and cosines of a token
 // are shared by its 2 H heads: the workgroup computes those of a run of tokens once, into LDS, while the loads of its
 // first tokens are in flight; the next token's loads follow the current one's last use of the registers.
-// Measured (hd 64, bf16): 65,536 tokens of 8 heads forward 74 us (5.4 TB/s), backward 112 us + 4 of dw sum (4.8 TB/s; four
+// Measured (hd 64, bf16): 65,536 tokens of 8 heads forward 71 us (5.7 TB/s), backward 112 us + 5 of dw sum (4.8 TB/s; four
 // waves per SIMD, at three it was 167), a large copy's rate on this card being 4.95; 32 x 1024 rows appended, a third of
-// them padding, 4 heads 19 us (3.8 TB/s); 512 sequences' single rows 5.3 us, the chain of past, page id and store.
+// them padding, 4 heads 19 us (3.8 TB/s); 512 sequences' single rows 6.0 us, the chain of past, page id and store.
 #include "common.h"
 
 #include <algorithm>
