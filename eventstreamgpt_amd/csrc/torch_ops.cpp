@@ -16,6 +16,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -619,11 +620,29 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
   }
 };
 
+// A leaf's gradient accumulator keeps the stream it was made on while any graph of the leaf lives. One of the default
+// stream cannot take part in a captured backward, and the failed capture would end the process: refused here instead.
+void refuse_capture_with(const Tensor& leaf) {
+  if (!leaf.defined() || !leaf.is_cuda() || !leaf.requires_grad() || !leaf.is_leaf()) return;
+  const auto acc = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (!acc || !acc->stream().has_value() || acc->stream()->id() != 0 || c10::hip::device_count() == 0) return;
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(reinterpret_cast<hipStream_t>(stream_of(leaf)), &st) != hipSuccess) (void)hipGetLastError();
+  TORCH_CHECK(st == hipStreamCaptureStatusNone, "eventstreamgpt_amd: qk_norm_rope is captured while an eager graph of the "
+              "same leaves, made on the default stream, is alive: its backward could not be captured (delete that graph, or "
+              "make it on the capturing stream)");
+}
+
 Tensor qk_norm_rope_autograd(const Tensor& qkv, const optional<Tensor>& q_w, const optional<Tensor>& k_w,
                              const optional<Tensor>& pos, const optional<Tensor>& inv_freq, int64_t H, double eps) {
   for (const auto* t : {&pos, &inv_freq})
     TORCH_CHECK_NOT_IMPLEMENTED(!t->has_value() || !(*t)->defined() || !(*t)->requires_grad(),
                                 "eventstreamgpt_amd: qk_norm_rope has no gradient for pos and inv_freq");
+  if (at::GradMode::is_enabled()) {
+    refuse_capture_with(qkv);
+    for (const auto* t : {&q_w, &k_w})
+      if (t->has_value()) refuse_capture_with(**t);
+  }
   return QkNormRope::apply(qkv, q_w, k_w, pos, inv_freq, H, eps);
 }
 

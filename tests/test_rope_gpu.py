@@ -245,6 +245,44 @@ def test_captured_and_replayed():
 
 
 @gpu
+def test_captured_backward_through_autograd():
+    """A graph with a layer's forward and backward through autograd. Captured while an eager graph of the same leaves lives
+    on the default stream it is refused, before anything is launched; without one every replay gives the eager bits."""
+    B, T, H, hd, R = 4, 40, 4, 64, 64
+    qkv, q_w, k_w, pos, f = inputs(B, T, H, hd, R, torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (qkv, q_w, k_w)]
+    dout = torch.randn(qkv.shape, device=DEV, dtype=qkv.dtype)
+
+    def step():
+        out = ops().qk_norm_rope(qkv, q_w, k_w, pos, f, H, EPS)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    eager = ops().qk_norm_rope(qkv, q_w, k_w, pos, f, H, EPS)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops().qk_norm_rope(qkv, q_w, k_w, pos, f, H, EPS)
+    eager.backward(dout)  # the graph that was there is none the worse
+    del eager
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        step()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        with torch.no_grad():
+            qkv.copy_(torch.randn_like(qkv))
+            q_w.add_(0.1)
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), i
+
+
+@gpu
 def test_empty_batches():
     qkv, q_w, k_w, pos, f = inputs(2, 3, 2, 16, 16, torch.float32)
     for B, T in ((0, 3), (2, 0)):
