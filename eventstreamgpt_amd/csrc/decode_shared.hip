@@ -846,32 +846,37 @@ int block_keys(int64_t hd, int dtype) {
                              : (hd <= 64 ? Walk<float, 2>::KB : Walk<float, 4>::KB);
 }
 
-// Whole or split, and how finely. The whole form saves the second launch and the parts' traffic but runs 16 rows a workgroup
-// and one workgroup of eight waves (above 64 dimensions two of four) a CU at a time; its rounds cost what its busiest wave's
-// chain of blocks costs (steps: those of the history and those of its trajectories' own rows). A tile is 16 rows, or 8 or 4
-// while there are fewer workgroups than CUs: the history is then read by more of them, out of L2, and each has fewer
-// trajectories (32x16 256+64: 16 rows 12.9, 8 rows 11.4). Measured in graph replays, whole / split us (groups x trajectories,
-// history + own rows, heads; hd 64 bf16 if not said):
+// Whole or split, and how finely. The whole form saves the second launch and the parts' traffic but runs 16 rows a
+// workgroup and one workgroup of eight waves (above 64 dimensions two of four) a CU at a time; its rounds cost what its
+// busiest wave's chain of blocks costs (steps: those of the history and those of its trajectories' own rows). A tile is
+// 16 rows, or 8 or 4 while there are fewer workgroups than CUs: the history is then read by more of them, out of L2,
+// and each has fewer trajectories (32x16 256+64: 16 rows 12.9, 8 rows 11.4). Measured in graph replays, whole / split
+// us (groups x trajectories, history + own rows, heads; hd 64 bf16 if not said):
 //   every block and trajectory has a wave of its own: 8x4 100+10 h4 6.8 / 7.9; 1x4 40+6 h4 f32 hd16 6.3 / 7.2
 //     (not so: 4x8 200+20 h4 f32 hd16 8.1 / 7.7)
-//   smaller tiles for half the CUs or more, and a chain of at most three: 32x16 256+64 h4 11.4 / 15.0; 32x8 256+64 h4 9.1 /
-//     11.5; 16x16 256+64 h4 f32 14.1 / 14.9 (a longer history: 4x16 1000+20 h8 12.3 / 9.9, 4x64 2048+32 h8 18.8 / 16.7)
-//   16-row tiles for every CU: by an estimate of both in us. Whole: 8 + 2.8 (f32 3.2) a step and round. Split: 14 + 1.2 (f32
-//     1.6) a step and workgroup of a CU, 32 rows a tile 1.6 (2.6), + 0.002 a block of own rows; all by a block's bytes / 16 KB.
-//     One full round, or short histories: 32x8 512+24 window 32 h8 8.3 / 14.3; 32x16 1000+20 h8 20.7 / 24.0, f32 39.6 / 42.6;
-//     32x16 512+128 h8 f32 55.0 / 64.7; 32x128 256+64 h4 62.6 / 70.0; 32x64 256+20 h4 hd128 27.6 / 56.6
-//     A round begun for a few workgroups: 33x8 1500+20 h8 35.5 / 29.0; 20x32 2000+20 h8 41.4 / 31.0; 24x40 2000+20 h8 f32 hd128
-//     240 / 174. Many row tiles over a long history: 8x64 two events 4096+20 h8 52.5 / 35.0, 32x40 two 3000+20 h8 114 / 85.0
+//   smaller tiles for half the CUs or more, and a chain of at most three: 32x16 256+64 h4 11.4 / 15.0; 32x8 256+64 h4
+//     9.1 / 11.5; 16x16 256+64 h4 f32 14.1 / 14.9 (a longer history: 4x16 1000+20 h8 12.3 / 9.9, 4x64 2048+32 h8 18.8 /
+//     16.7)
+//   16-row tiles for every CU: by an estimate of both in us. Whole: 8 + 2.8 (f32 3.2) a step and round. Split: 14 + 1.2
+//     (f32 1.6) a step and workgroup of a CU, 32 rows a tile 1.6 (2.6), + 0.002 a block of own rows; all by a block's
+//     bytes / 16 KB.
+//     One full round, or short histories: 32x8 512+24 window 32 h8 8.3 / 14.3; 32x16 1000+20 h8 20.7 / 24.0, f32 39.6 /
+//       42.6; 32x16 512+128 h8 f32 55.0 / 64.7; 32x128 256+64 h4 62.6 / 70.0; 32x64 256+20 h4 hd128 27.6 / 56.6
+//     A round begun for a few workgroups: 33x8 1500+20 h8 35.5 / 29.0; 20x32 2000+20 h8 41.4 / 31.0; 24x40 2000+20 h8
+//       f32 hd128 240 / 174. Many row tiles over a long history: 8x64 two events 4096+20 h8 52.5 / 35.0, 32x40 two
+//       3000+20 h8 114 / 85.0
 //     One wave's chain of own rows: 64x1 512+400 h8 34.9 / 24.9, 64x2 39.3 / 34.8
 // Without a history the split form's waves are the whole of it, and write directly where one chunk holds a trajectory.
-// The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 55.8 / 58.8, 8x8 8192+32 h8 f32 50.7 /
-// 52.2, 16x4 1024+33 h4 f32 15.0 / 18.2, 4x64 2048+32 h8 16.9 / 20.1 (more parts cost more joins); own rows at 1,024 waves:
-// 16x16 256+64 f32 15.7 against 19.7 at 4,096. In f32 up to 32 dimensions a workgroup has little in flight, and two a CU pay:
-// 8x32 8192+32 h8 hd32 55.1 -> 42.2, 2x64 4096+32 h8 hd16 16.9 -> 15.0 (bf16 19.3 -> 20.6, 10.7 -> 10.6).
-// History tiles of 32 rows halve the reads but leave half the workgroups to share a history; they pay where each wave still has
-// 256 keys. 16 / 32 rows: 24x40 2000+20 h8 51.3 / 46.0, 20x32 2000 32.2 / 30.9, 4x32 16384 h8 f32 78.6 / 66.1, 16x32 4096 f32
-// 83.4 / 71.4; fewer: 4x20 1000 h4 9.1 / 10.8, 1x40 6000 h8 13.3 / 14.4, 8x32 2048 f32 27.8 / 28.4. At 128 dimensions (f32: above
-// 64) two accumulators leave one wave a SIMD: 24x40 2000 h8 77.3 / 96.4, 1x40 6000 18.5 / 25.7.
+// The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 55.8 / 58.8, 8x8 8192+32 h8 f32
+// 50.7 / 52.2, 16x4 1024+33 h4 f32 15.0 / 18.2, 4x64 2048+32 h8 16.9 / 20.1 (more parts cost more joins); own rows at
+// 1,024 waves: 16x16 256+64 f32 15.7 against 19.7 at 4,096. In f32 up to 32 dimensions a workgroup has little in
+// flight, and two a CU pay: 8x32 8192+32 h8 hd32 55.1 -> 42.2, 2x64 4096+32 h8 hd16 16.9 -> 15.0 (bf16 19.3 -> 20.6,
+// 10.7 -> 10.6).
+// History tiles of 32 rows halve the reads but leave half the workgroups to share a history; they pay where each wave
+// still has 256 keys. 16 / 32 rows: 24x40 2000+20 h8 51.3 / 46.0, 20x32 2000 32.2 / 30.9, 4x32 16384 h8 f32 78.6 /
+// 66.1, 16x32 4096 f32 83.4 / 71.4; fewer: 4x20 1000 h4 9.1 / 10.8, 1x40 6000 h8 13.3 / 14.4, 8x32 2048 f32 27.8 /
+// 28.4. At 128 dimensions (f32: above 64) two accumulators leave one wave a SIMD: 24x40 2000 h8 77.3 / 96.4, 1x40 6000
+// 18.5 / 25.7.
 SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap, int64_t cap,
                        int64_t window, int dtype) {
   SharedPlan p{};
@@ -904,7 +909,8 @@ SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, 
   const double a_cu = 0.5 * std::max<int64_t>(2, cdiv(2 * p.units, kCus));  // workgroups
   const double split_us = 14 + block * ((p.NT == 2 ? (bf ? 1.6 : 2.6) : (bf ? 1.2 : 1.6)) * a_cu * (p.pchunk / round) +
                                         0.002 * (double)(S * H) * cdiv(sspan, kb));
-  p.whole = pspan > 0 && (cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw || (tr == 16 && units >= kCus && whole_us <= split_us) ||
+  p.whole = pspan > 0 && (cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw ||
+                          (tr == 16 && units >= kCus && whole_us <= split_us) ||
                           (units >= kCus / 2 && steps <= 1 && own_steps <= 2));
   if (p.whole) {
     p.tr = (int)tr;

@@ -311,12 +311,18 @@ def test_bounds_wider_than_the_lengths():
 
 @gpu
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("c", [(2, 33, 1, 8, 64, 16, 300, 20, 0), (2, 25, 2, 8, 20, 64, 700, 20, 0), (1, 70, 1, 16, 32, 16, 90, 9, 0)],
-                         ids=str)
+@pytest.mark.parametrize("c", [(2, 33, 1, 8, 64, 16, 300, 20, 0), (2, 25, 2, 8, 20, 64, 700, 20, 0), (1, 70, 1, 16, 32, 16, 90, 9, 0),
+                               (2, 17, 3, 8, 96, 16, 200, 12, 0)], ids=str)
 def test_tiles_of_32_rows_over_long_bounds(c, dt):
-    """Bounds that a long history would need (the work is split by them) over short ones: f32 takes 32 rows a tile too."""
-    x = Case(*c, dt=dt) if c[4] % 8 == 0 or dt == F32 else Case(*c[:4], 24, *c[5:], dt=dt)
+    """Bounds that a long history would need (the work is split by them) over short ones, which makes the tiles 32 rows
+    high; padded rows; NaN in the used pages' unused rows."""
+    x = Case(*(c if c[4] % 8 == 0 or dt == F32 else (*c[:4], 24, *c[5:])), dt=dt, masked=c[2] > 1)
     want = x.oracle()
+    for table, lens in ((x.prefix_table, x.prefix_lens), (x.table, torch.tensor([x.own_row(s, x.Lq) for s in range(x.S)]))):
+        for pages, n in zip(table.long(), lens.tolist()):
+            for i, page in enumerate(pages.tolist()):
+                x.kp[page, :, min(max(n - i * x.ps, 0), x.ps):] = math.nan
+                x.vp[page, :, min(max(n - i * x.ps, 0), x.ps):] = math.nan
     x.prefix_table = torch.cat([x.prefix_table, torch.full((x.G, 16384 // x.ps), -1).int()], 1)
     cap = x.prefix_table.shape[1] * x.ps
     got = x.run(prefix_cap=cap)
