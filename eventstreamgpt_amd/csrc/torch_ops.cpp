@@ -573,10 +573,10 @@ std::tuple<Tensor, Tensor> qk_norm_rope_bwd(const Tensor& dout_, const Tensor& q
   Tensor dqkv = at::empty(qkv.sizes(), qkv.options());
   Tensor dw = at::empty({r.q_w.defined() ? 2 : 0, hd}, qkv.options().dtype(at::kFloat));
   const size_t nb = r.q_w.defined() ? esgpt_qk_norm_rope_bwd_workspace(N, H, hd, r.R, dt) : 0;
-  Tensor ws = at::empty({(int64_t)nb}, qkv.options().dtype(at::kByte));
+  Tensor ws = nb ? at::empty({(int64_t)nb}, qkv.options().dtype(at::kByte)) : Tensor();
   check(esgpt_qk_norm_rope_bwd(dout.data_ptr(), qkv.data_ptr(), fptr(r.q_w), fptr(r.k_w), vptr(r.pos), r.pos_dtype,
                                fptr(r.inv_freq), r.R, N, H, hd, (float)eps, dqkv.data_ptr(), ptr<float>(dw),
-                               ws.data_ptr(), nb, dt, stream_of(qkv)),
+                               nb ? ws.data_ptr() : nullptr, nb, dt, stream_of(qkv)),
         "qk_norm_rope_bwd");
   return {dqkv, dw};
 }
@@ -740,14 +740,46 @@ Tensor attn_decode_shared(const Tensor& q_, const Tensor& k_pages, const Tensor&
   if (o.numel() == 0) return o;
   const int dt = dtype_code(q.scalar_type());
   const size_t nb = esgpt_attn_decode_shared_workspace(G, S, Lq, H, hd, prefix_cap, cap, window, dt);
-  Tensor ws = at::empty({(int64_t)nb}, q.options().dtype(at::kByte));
+  Tensor ws = nb ? at::empty({(int64_t)nb}, q.options().dtype(at::kByte)) : Tensor();
   check(esgpt_attn_decode_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.size(0), ps,
                                  ptr<const int32_t>(ptab), pre ? ptab.size(1) : 0, ptr<const int32_t>(plen), G,
                                  ptr<const int32_t>(page_table), page_table.size(1), ptr<const int32_t>(past),
                                  m.defined() ? ptr<const uint8_t>(m) : nullptr, o.data_ptr(), S, Lq, H, hd, prefix_cap,
-                                 cap, window, dt, ws.data_ptr(), nb, e, stream_of(q)),
+                                 cap, window, dt, nb ? ws.data_ptr() : nullptr, nb, e, stream_of(q)),
         "attn_decode_shared");
   return o;
+}
+
+// The paged cache is for generation: gradients are refused, and the call goes on below autograd.
+template <typename... Ts>
+void no_gradient(const char* what, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled() || !(ts.requires_grad() || ...), "eventstreamgpt_amd: ", what,
+                              " is for generation and has no gradient (run under torch.no_grad())");
+}
+
+Tensor kv_append_paged_autograd(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                                const Tensor& past, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
+                                const optional<Tensor>& k_w, const optional<Tensor>& pos,
+                                const optional<Tensor>& inv_freq, double eps, const Tensor& err) {
+  auto t = [](const optional<Tensor>& x) { return x.has_value() ? *x : Tensor(); };
+  no_gradient("kv_append_paged", qkv, k_pages, v_pages, t(q_w), t(k_w), t(pos), t(inv_freq));
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("esgpt::kv_append_paged", "")
+                       .typed<decltype(kv_append_paged)>();
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err);
+}
+
+Tensor attn_decode_shared_autograd(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                                   const optional<Tensor>& prefix_table, const optional<Tensor>& prefix_lens,
+                                   const Tensor& page_table, const Tensor& past, const optional<Tensor>& row_mask,
+                                   int64_t prefix_cap, int64_t cap, int64_t window, const Tensor& err) {
+  no_gradient("attn_decode_shared", q, k_pages, v_pages);
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("esgpt::attn_decode_shared", "")
+                       .typed<decltype(attn_decode_shared)>();
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, past, row_mask, prefix_cap, cap, window, err);
 }
 
 // ---- output-layer losses -------------------------------------------------------------------------------------------
@@ -1434,4 +1466,8 @@ TORCH_LIBRARY_IMPL(esgpt, CUDA, m) {
   m.impl("adamw_dev", &adamw_dev);
 }
 
-TORCH_LIBRARY_IMPL(esgpt, Autograd, m) { m.impl("qk_norm_rope", &qk_norm_rope_autograd); }
+TORCH_LIBRARY_IMPL(esgpt, Autograd, m) {
+  m.impl("qk_norm_rope", &qk_norm_rope_autograd);
+  m.impl("kv_append_paged", &kv_append_paged_autograd);
+  m.impl("attn_decode_shared", &attn_decode_shared_autograd);
+}

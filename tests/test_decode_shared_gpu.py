@@ -578,6 +578,9 @@ def test_fake_tensors():
     out = o.attn_decode_shared(q, kp, kp, None, None, torch.empty(3, 1, **m), torch.empty(3, **m), None, 0, 16, 0,
                                torch.empty(2, device="meta", dtype=torch.int64))
     assert out.shape == q.shape
+    with pytest.raises(NotImplementedError, match="no_grad"):
+        o.attn_decode_shared(q.requires_grad_(), kp, kp, None, None, torch.empty(3, 1, **m), torch.empty(3, **m), None, 0,
+                             16, 0, torch.empty(2, device="meta", dtype=torch.int64))
 
 
 def test_paged_cache_hands_out_each_page_once():

@@ -517,6 +517,13 @@ def test_fake_tensors_and_autograd_formula():
                           torch.empty(2, device="meta", dtype=torch.int32), None, None, None, None, None, EPS,
                           torch.empty(2, device="meta", dtype=torch.int64))
     assert q.shape == (2, 3, 32) and q.dtype == torch.bfloat16
+    args = (kp, kp.clone(), torch.empty(2, 2, device="meta", dtype=torch.int32),
+            torch.empty(2, device="meta", dtype=torch.int32), None, q_w, k_w, pos, f, EPS,
+            torch.empty(2, device="meta", dtype=torch.int64))
+    with pytest.raises(NotImplementedError, match="no_grad"):  # the weights ask for a gradient
+        o.kv_append_paged(qkv.detach(), *args)
+    with torch.no_grad():
+        assert o.kv_append_paged(qkv, *args).shape == q.shape
 
 
 def test_error_flag_raises_index_error():
