@@ -852,8 +852,13 @@ int block_keys(int64_t hd, int dtype) {
 // 16 rows, or 8 or 4 while there are fewer workgroups than CUs: the history is then read by more of them, out of L2,
 // and each has fewer trajectories (32x16 256+64: 16 rows 12.9, 8 rows 11.4). Measured in graph replays, whole / split
 // us (groups x trajectories, history + own rows, heads; hd 64 bf16 if not said):
-//   every block and trajectory has a wave of its own: 8x4 100+10 h4 6.8 / 7.9; 1x4 40+6 h4 f32 hd16 6.3 / 7.2
-//     (not so: 4x8 200+20 h4 f32 hd16 8.1 / 7.7)
+//   the busiest wave's chain of blocks is short: one; two in bf16 if half the waves have no history; up to 32 dimensions
+//     one more, three in bf16. In a graph 8x4 100+10 h4 6.8 / 7.9; 1x4 40+6 h4 f32 hd16 6.3 / 7.2; 4x4 100+100 h4 8.4 /
+//     9.1; 8x30 3+5 h1 hd128 8.4 / 8.7; 4x16 500+60 h4 hd32 7.8 / 7.9; 4x8 200+20 h4 f32 hd16 8.1 / 7.7; 5x2 691+109 h8
+//     hd16 8.2 / 7.6; 3x5 900+50 h4 hd16 8.6 / 7.6. A call that is not in a graph pays 3 us of host time for the second
+//     launch and its workspace: the last four 7.8 / 10.4, 8.1 / 10.6, 8.3 / 10.7, 8.7 / 10.6. Longer chains lose: 8x8
+//     400+40 h4 9.4 / 8.6, 1x8 600+30 h8 9.8 / 8.4, 16x4 87+288 h2 hd24 10.0 / 7.6, 8x4 300+30 h4 hd128 11.9 / 9.8, f32
+//     4x16 256+64 h4 13.2 / 11.2, 2x13 106+189 h5 hd16 12.2 / 7.9
 //   smaller tiles for half the CUs or more, and a chain of at most three: 32x16 256+64 h4 11.4 / 15.0; 32x8 256+64 h4
 //     9.1 / 11.5; 16x16 256+64 h4 f32 14.1 / 14.9 (a longer history: 4x16 1000+20 h8 12.3 / 9.9, 4x64 2048+32 h8 18.8 /
 //     16.7)
@@ -909,7 +914,12 @@ SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, 
   const double a_cu = 0.5 * std::max<int64_t>(2, cdiv(2 * p.units, kCus));  // workgroups
   const double split_us = 14 + block * ((p.NT == 2 ? (bf ? 1.6 : 2.6) : (bf ? 1.2 : 1.6)) * a_cu * (p.pchunk / round) +
                                         0.002 * (double)(S * H) * cdiv(sspan, kb));
-  p.whole = pspan > 0 && (cdiv(pspan, kb) + seqs * cdiv(sspan, kb) <= nw ||
+  const int64_t hist = cdiv(pspan, kb);
+  int64_t chain = 0;
+  for (int64_t w = 0; w < nw; ++w)
+    chain = std::max(chain, cdiv(std::max<int64_t>(hist - w, 0), nw) +
+                                cdiv(std::max<int64_t>(seqs - (nw - 1 - w), 0), nw) * cdiv(sspan, kb));
+  p.whole = pspan > 0 && (chain <= 1 + (hd <= 32) + (bf && (hd <= 32 || 2 * hist <= nw)) ||
                           (tr == 16 && units >= kCus && whole_us <= split_us) ||
                           (units >= kCus / 2 && steps <= 1 && own_steps <= 2));
   if (p.whole) {
