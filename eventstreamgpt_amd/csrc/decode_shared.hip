@@ -291,8 +291,47 @@ struct Walk {
     }
   }
 
-  // P.V of a partly masked block key by key: a key adds nothing (not even 0 x infinity) to the rows that do not see it.
-  // Reads the values again; only a walk that has met a value that is not finite comes here.
+  // O += P.V of one block whose V tile is in LDS, P as the sum of two bf16: its upper half and what that leaves (off by
+  // 2^-15 of P; the 2^-20 keep the second part above zero, so that a visible infinity stays one). One part alone, off by
+  // 2^-8, is as coarse as the output's own rounding: 32 x 16 over 256 + 64 was off by 1.78e-3 of the result, the plain
+  // form in f32 by 1.66e-3. The second part costs three vector operations a probability and as many products as the first.
+  template <int NT>
+  __device__ __forceinline__ void pv(State<NT, DT>& st, const float (&p)[NT][4 * KT]) const {
+    const __bf16* vr = vt + (4 * g + (c >> 2)) * LD + 4 * (c & 3);
+#pragma unroll
+    for (int u = 0; u < KT; u += 2) {
+      bf16x8 ph[NT], pl[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float pi = p[t][4 * u + i];
+          const uint32_t hi = __float_as_uint(pi) & 0xFFFF0000u;
+          ph[t][i] = __builtin_bit_cast(__bf16, (uint16_t)(hi >> 16));
+          pl[t][i] = (__bf16)fmaf(pi, 1.f + 0x1p-20f, -__uint_as_float(hi));
+        }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        typedef __attribute__((address_space(3))) bf16x4* lds4;
+        const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * u * LD + 16 * d));
+        const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * (u + 1) * LD + 16 * d));
+        bf16x8 vf;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          vf[i] = x[i];
+          vf[4 + i] = y[i];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph[t], st.acc[t][d], 0, 0, 0);
+          st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[t], st.acc[t][d], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  // P.V of a partly masked block key by key: a key adds nothing (not even 0 x infinity) to the rows
+  // that do not see it. Reads the values again; only a walk that has met a value that is not finite comes here.
   __device__ __forceinline__ void masked_pv(const Offsets& of, int slot, const float (&p)[4 * KT], f32x4 (&o)[DT], int k0,
                                             int lo, int hi) const {
 #pragma nounroll
@@ -306,7 +345,7 @@ struct Walk {
       for (int j = 1; j < 4 * KT; ++j) pi = i == j ? p[j] : pi;
 #pragma nounroll
       for (int gg = 0; gg < 4; ++gg) {
-        const float pk = to_f32(from_f32<T>(__shfl(pi, 16 * gg + c, 64)));
+        const float pk = __shfl(pi, 16 * gg + c, 64);
         const int row = 4 * gg + (i & 3), key = k0 + (i & ~3) * 4 + row;
         if (key < lo || key >= hi) continue;
 #pragma unroll
@@ -446,31 +485,7 @@ struct Walk {
 #pragma unroll
         for (int t = 0; t < NT; ++t) masked_pv(now.of, now.slot, p[t], st.acc[t], k0, lo[t], hi[t]);
       } else if constexpr (kBf16) {
-        // P in bf16 for the matrix product (as esgpt_attn_fwd and esgpt_attn_decode round it; the sums stay f32)
-        const __bf16* vr = vt + (4 * g + (c >> 2)) * LD + 4 * (c & 3);
-#pragma unroll
-        for (int u = 0; u < KT; u += 2) {
-          bf16x8 pf[NT];
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pf[t][i] = (__bf16)p[t][4 * u + i];
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            typedef __attribute__((address_space(3))) bf16x4* lds4;
-            const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * u * LD + 16 * d));
-            const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vr + 16 * (u + 1) * LD + 16 * d));
-            bf16x8 vf;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              vf[i] = x[i];
-              vf[4 + i] = y[i];
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-              st.acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], st.acc[t][d], 0, 0, 0);
-          }
-        }
+        pv(st, p);
       } else {
 #pragma unroll
         for (int u = 0; u < KT; ++u) {

@@ -607,3 +607,59 @@ def test_paged_cache_hands_out_each_page_once():
     for ps in (8, 24, 1 << 17):
         with pytest.raises(ValueError, match="page size"):
             PagedKV(2, ps, 2, 32, torch.float32, "cpu")
+
+
+# ------------------------------------------------------------------------------------- accuracy of bf16 probabilities
+def tight(x, got, want, extra=2.0**-15 + 2.0**-20):
+    """As Case.check, but nothing is granted for P in bf16: P enters the product as its upper half and, rounded (2^-8), what
+    that leaves (below 2^-7 of P) and 2^-20 of P. The output's half step is of the computed value."""
+    o, mag, size = want
+    got = got.cpu().double().view(x.S, x.Lq, x.H, x.hd)
+    rel = 2 * (x.hd + 8) * U * size + (16 + (x.P + x.s) / 16 + 64) * U
+    off = (rel + extra) * mag
+    lim = off + 2.0**-8 * (o.abs() + off)
+    bad = ~((got - o).abs() <= lim)
+    assert not bad.any(), (bad.sum().item(), ((got - o).abs() / lim.clamp_min(1e-30)).max().item())
+
+
+@gpu
+@pytest.mark.parametrize("c", [
+    (16, 9, 1, 8, 64, 32, 100, 40, 0), (32, 3, 2, 4, 128, 16, 70, 20, 0), (16, 3, 1, 8, 96, 16, 90, 12, 20),
+    (33, 2, 1, 8, 40, 16, 20, 5, 0), (1, 4, 1, 4, 16, 16, 40, 6, 0),                # whole
+    (1, 6, 1, 2, 64, 64, 9001, 700, 0), (2, 3, 1, 2, 24, 16, 0, 19, 0), (1, 40, 2, 1, 64, 64, 5000, 40, 700),
+    (64, 20, 1, 16, 16, 64, 1100, 8, 0),                                            # split, tiles of 16 and 32 rows
+], ids=str)
+def test_bf16_probabilities_keep_sixteen_bits(c):
+    """Values that cancel: a probability rounded to bf16 would be off by more than the small result's own rounding."""
+    x = Case(*c, dt=BF16, share=c[0] == 64)
+    if c[0] == 64:  # the oracle's time: a few sequences
+        got = x.run()
+        y = Case(*c, dt=BF16, share=True)
+        for s in (0, 700, 1279):
+            y.S = y.G = y.n = 1
+            y.prefix_table, y.prefix_lens = x.prefix_table[s // 20: s // 20 + 1], x.prefix_lens[s // 20: s // 20 + 1]
+            y.table, y.past, y.q = x.table[s: s + 1], x.past[s: s + 1], x.q[s: s + 1]
+            tight(y, got[s: s + 1], y.oracle())
+        return
+    tight(x, x.run(), x.oracle())
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", [(2, 5, 1, 2, 64, 64, 300, 21, 0), (16, 5, 1, 8, 64, 64, 300, 21, 0), (1, 20, 1, 2, 96, 32, 700, 9, 0)],
+                         ids=str)
+def test_a_visible_infinity_stays_one(c, dt):
+    """Where a row sees an infinite value with a probability above zero its result is that infinity, and the rest of
+    the row is as accurate as without it."""
+    x = Case(*c, dt=dt, ragged=False)
+    want = x.oracle()
+    for j, d, v in ((3, 5, math.inf), (130, 6, -math.inf)):
+        for gr in range(x.G):
+            x.vp[x.prefix_table[gr, j // x.ps], 1, j % x.ps, d] = v
+    got = x.run().view(x.S, x.Lq, x.H, x.hd)
+    assert (got[:, :, 1, 5] == math.inf).all() and (got[:, :, 1, 6] == -math.inf).all()
+    mask = torch.ones(got.shape, dtype=torch.bool)
+    mask[:, :, 1, 5:7] = False
+    o, mag, size = want
+    got = torch.where(mask, got.cpu().double(), torch.zeros(()).double())
+    tight(x, got, (o * mask, mag * mask, size), *(() if dt == BF16 else (0.0,)))
