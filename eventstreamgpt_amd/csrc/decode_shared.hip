@@ -73,6 +73,10 @@ __device__ __forceinline__ float xsum(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+// e^{s - m}, m >= s the running maximum (0 while there is none). The difference comes first: it is exact near the maximum,
+// where s log2(e) - (m log2(e) rounded) would be off by 2^-24 of m, a factor beyond f32 for scores above 10^9.
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ float weight(float s, float base) { return __builtin_amdgcn_exp2f((s - base) * kLog2e); }
 // A value that is the same in every lane, in a scalar register: buffer descriptors, page places and loop bounds that the
 // compiler finds in vector registers cost a loop over the lanes at each use.
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -465,9 +469,9 @@ struct Walk {
 #pragma unroll
         for (int i = 1; i < 4 * KT; ++i) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
         const float mn = fmaxf(st.m[t], xmax(mx));
-        const float mc = mn == -INFINITY ? 0.f : mn * kLog2e;
+        const float mc = base_of(mn);
         if (__any(mn != st.m[t])) {
-          const float f = __builtin_amdgcn_exp2f(fmaf(st.m[t], kLog2e, -mc));
+          const float f = weight(st.m[t], mc);
           st.l[t] *= f;
 #pragma unroll
           for (int d = 0; d < DT; ++d) st.acc[t][d] *= f;
@@ -476,7 +480,7 @@ struct Walk {
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4 * KT; ++i) {
-          p[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], kLog2e, -mc));
+          p[t][i] = weight(s[t][i >> 2][i & 3], mc);
           sum += p[t][i];
         }
         st.l[t] += sum;
@@ -588,14 +592,14 @@ struct Join {
       if (d0 == 0) {
         for (int u = 0; u < NW; ++u) M = fmaxf(M, jl[u * 16 + row] == 0.f ? -INFINITY : jm[u * 16 + row]);
       }
-      const float mc = M == -INFINITY ? 0.f : M * kLog2e;
+      const float mc = base_of(M);
       const int d = d0 + 4 * (threadIdx.x & 15);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       float Ls = 0.f;
       for (int u = 0; u < NW; ++u) {
         const float lu = jl[u * 16 + row];
         if (lu == 0.f) continue;  // this wave saw nothing for the row
-        const float f = __builtin_amdgcn_exp2f(fmaf(jm[u * 16 + row], kLog2e, -mc));
+        const float f = weight(jm[u * 16 + row], mc);
         Ls = fmaf(lu, f, Ls);
         if (d - d0 >= W) continue;
         const float4 y = *reinterpret_cast<const float4*>(jo + (u * 16 + row) * OLD + d - d0);
@@ -822,8 +826,8 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a, int64_t 
   const float2* ml = reinterpret_cast<const float2*>(a.ml) + rh * a.NP;
   const float2 own = lane < a.NP ? ml[lane] : make_float2(-INFINITY, 0.f);  // NP <= 64
   const float M = wave_max(own.y == 0.f ? -INFINITY : own.x);
-  const float mc = M == -INFINITY ? 0.f : M * kLog2e;
-  const float f = own.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(fmaf(own.x, kLog2e, -mc));
+  const float mc = base_of(M);
+  const float f = own.y == 0.f ? 0.f : weight(own.x, mc);
   const float L = wave_sum(own.y == 0.f ? 0.f : own.y * f);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int p0 = 0; p0 < a.NP; p0 += nsub) {

@@ -663,3 +663,31 @@ def test_a_visible_infinity_stays_one(c, dt):
     o, mag, size = want
     got = torch.where(mask, got.cpu().double(), torch.zeros(()).double())
     tight(x, got, (o * mask, mag * mask, size), *(() if dt == BF16 else (0.0,)))
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", [(1, 4, 1, 1, 64, 16, 120, 6, 0), (16, 4, 1, 8, 64, 32, 90, 7, 0), (1, 40, 1, 2, 96, 64, 900, 9, 0),
+                               (2, 3, 2, 2, 32, 16, 0, 100, 0), (1, 6, 1, 2, 64, 64, 9001, 70, 0)], ids=str)
+def test_scores_of_any_size(c, dt):
+    """Scores up to 2^110 whose smallest distance is far above 1: the row is its largest key's value, bit for bit
+    (one probability of 1, the others 0; in bf16 the parts of 1 are 1 and 2^-20, far below half a step)."""
+    x = Case(*c, dt=dt, ragged=False)
+    g = torch.Generator().manual_seed(1)
+    for scale in (2.0**29, -(2.0**29), 2.0**33, 2.0**47, 2.0**101):
+        for top in (191, 254):
+            # key j is a_j in each dimension (integers, exact in bf16), the query `scale` in the first one and 0 elsewhere
+            a = torch.randint(1, top - 1, x.kp.shape[:3], generator=g)
+            x.kp = a[..., None].to(dt).expand(x.kp.shape).clone()
+            x.q = torch.zeros_like(x.q).view(x.S, x.Lq, x.H, x.hd)
+            x.q[..., 0] = scale
+            x.q = x.q.view(x.S, x.Lq, -1)
+            # one own row of every sequence outdoes all others
+            for s in range(x.S):
+                r = int(x.past[s]) // 2
+                x.kp[x.table[s, r // x.ps], :, r % x.ps] = top if scale > 0 else 0
+            got = x.run().view(x.S, x.Lq, x.H, x.hd).cpu()
+            for s in range(x.S):
+                r = int(x.past[s]) // 2
+                want = x.vp[x.table[s, r // x.ps], :, r % x.ps].expand(x.Lq, -1, -1)
+                assert torch.equal(got[s], want), (scale, top, s)
