@@ -586,6 +586,15 @@ std::tuple<Tensor, Tensor> qk_norm_rope_bwd(const Tensor& dout_, const Tensor& q
   return {dqkv, dw};
 }
 
+std::tuple<Tensor, Tensor> call_bwd(const Tensor& dout, const Tensor& qkv, const optional<Tensor>& q_w,
+                                    const optional<Tensor>& k_w, const optional<Tensor>& pos,
+                                    const optional<Tensor>& inv_freq, int64_t H, double eps) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("esgpt::qk_norm_rope_bwd", "")
+                       .typed<decltype(qk_norm_rope_bwd)>();
+  return op.call(dout, qkv, q_w, k_w, pos, inv_freq, H, eps);
+}
+
 // d qkv from the raw buffer (the norms are recomputed), d q_w and d k_w summed in a fixed order. In C++: one layer's
 // forward and backward take 24 us on the device at the 256-wide model's training batch, and a formula registered from
 // Python costs an eager step 70 us of host time.
@@ -607,15 +616,12 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
                                                  torch::autograd::variable_list grads) {
     torch::autograd::variable_list out(7);
     if (!grads[0].defined()) return out;
-    static auto op = c10::Dispatcher::singleton()
-                         .findSchemaOrThrow("esgpt::qk_norm_rope_bwd", "")
-                         .typed<decltype(qk_norm_rope_bwd)>();
     optional<at::AutoDispatchBelowADInplaceOrView> guard;  // unless this backward is itself recorded: straight to the kernel
     if (!at::GradMode::is_enabled()) guard.emplace();
     auto s = ctx->get_saved_variables();
     auto o = [](const Tensor& x) { return x.defined() ? optional<Tensor>(x) : optional<Tensor>(); };
-    auto [dqkv, dw] = op.call(grads[0], s[0], o(s[1]), o(s[2]), o(s[3]), o(s[4]), ctx->saved_data["H"].toInt(),
-                              ctx->saved_data["eps"].toDouble());
+    auto [dqkv, dw] = call_bwd(grads[0], s[0], o(s[1]), o(s[2]), o(s[3]), o(s[4]), ctx->saved_data["H"].toInt(),
+                               ctx->saved_data["eps"].toDouble());
     out[0] = dqkv;
     if (s[1].defined()) {
       out[1] = dw.select(0, 0);
@@ -624,6 +630,40 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
     return out;
   }
 };
+
+// Whether a derivative through t would be asked for: recorded, or carried along in forward mode.
+bool tracked(const Tensor& t) {
+  return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(/*level=*/0).defined());
+}
+
+// The backward as an operator of its own, or recorded (create_graph): its results are right, and a second derivative
+// through them, which has no formula, raises instead of counting as zero.
+struct QkNormRopeBwd : public torch::autograd::Function<QkNormRopeBwd> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, const Tensor& dout, const Tensor& qkv,
+                                                const optional<Tensor>& q_w, const optional<Tensor>& k_w,
+                                                const optional<Tensor>& pos, const optional<Tensor>& inv_freq, int64_t H,
+                                                double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [dqkv, dw] = call_bwd(dout, qkv, q_w, k_w, pos, inv_freq, H, eps);
+    return {dqkv, dw};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "eventstreamgpt_amd: qk_norm_rope has no second derivative");
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope_bwd_autograd(const Tensor& dout, const Tensor& qkv, const optional<Tensor>& q_w,
+                                                     const optional<Tensor>& k_w, const optional<Tensor>& pos,
+                                                     const optional<Tensor>& inv_freq, int64_t H, double eps) {
+  bool any = tracked(dout) || tracked(qkv);
+  for (const auto* t : {&q_w, &k_w, &pos, &inv_freq}) any = any || (t->has_value() && tracked(**t));
+  if (!any) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_bwd(dout, qkv, q_w, k_w, pos, inv_freq, H, eps);
+  }
+  auto r = QkNormRopeBwd::apply(dout, qkv, q_w, k_w, pos, inv_freq, H, eps);
+  return {r[0], r[1]};
+}
 
 // A leaf's gradient accumulator keeps the stream it was made on while any graph of the leaf lives. One of the default
 // stream cannot take part in a captured backward, and the failed capture would end the process: refused here instead.
@@ -1473,6 +1513,7 @@ TORCH_LIBRARY_IMPL(esgpt, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(esgpt, Autograd, m) {
   m.impl("qk_norm_rope", &qk_norm_rope_autograd);
+  m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd_autograd);
   m.impl("kv_append_paged", &kv_append_paged_autograd);
   m.impl("attn_decode_shared", &attn_decode_shared_autograd);
 }

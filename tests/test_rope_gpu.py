@@ -532,3 +532,27 @@ def test_error_flag_raises_index_error():
 
     with pytest.raises(IndexError, match="paged cache"):
         raise_for_error(L.FLAG_BAD_PAGE, 0)
+
+
+def test_second_derivatives_are_refused():
+    """A recorded backward gives its gradients; a derivative of those raises, and so does one through the backward
+    operator itself. An unrecorded call of it is not in any graph."""
+    o = ops()
+    qkv, q_w, k_w, pos, f = inputs(2, 3, 2, 16, 16, torch.float32, dev="meta")
+    leaves = [t.requires_grad_() for t in (qkv, q_w, k_w)]
+    for leaf in leaves:
+        out = o.qk_norm_rope(qkv, q_w, k_w, pos, f, 2, EPS)
+        grads = torch.autograd.grad(out.square().sum(), leaves, create_graph=True)
+        assert [g.shape for g in grads] == [t.shape for t in leaves]
+        with pytest.raises(NotImplementedError, match="second derivative"):
+            torch.autograd.grad(sum(g.sum() for g in grads), leaf)
+    dout = torch.empty_like(qkv).requires_grad_()
+    for kw in (dict(dout=dout), dict(dout=dout.detach())):
+        dqkv, dw = o.qk_norm_rope_bwd(kw["dout"], qkv, q_w, k_w, pos, f, 2, EPS)
+        with pytest.raises(NotImplementedError, match="second derivative"):
+            (dqkv.sum() + dw.sum()).backward()
+    with torch.no_grad():
+        dqkv, dw = o.qk_norm_rope_bwd(dout, qkv, q_w, k_w, pos, f, 2, EPS)
+    assert not dqkv.requires_grad and not dw.requires_grad and dw.shape == (2, 16)
+    dqkv, dw = o.qk_norm_rope_bwd(*(t.detach() for t in (dout, qkv)), None, None, pos, f, 2, EPS)
+    assert not dqkv.requires_grad and dw.shape == (0, 16)
