@@ -795,11 +795,12 @@ Tensor attn_decode_shared(const Tensor& q_, const Tensor& k_pages, const Tensor&
   return o;
 }
 
-// The paged cache is for generation: gradients are refused, and the call goes on below autograd.
+// The paged cache is for generation: gradients of either mode are refused, and the call goes on below autograd.
 template <typename... Ts>
 void no_gradient(const char* what, const Ts&... ts) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled() || !(ts.requires_grad() || ...), "eventstreamgpt_amd: ", what,
-                              " is for generation and has no gradient (run under torch.no_grad())");
+  TORCH_CHECK_NOT_IMPLEMENTED(!(tracked(ts) || ...), "eventstreamgpt_amd: ", what,
+                              " is for generation and has no gradient (run under torch.no_grad(), on tensors without a "
+                              "forward-mode tangent)");
 }
 
 Tensor kv_append_paged_autograd(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,

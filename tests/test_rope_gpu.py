@@ -556,3 +556,35 @@ def test_second_derivatives_are_refused():
     assert not dqkv.requires_grad and not dw.requires_grad and dw.shape == (2, 16)
     dqkv, dw = o.qk_norm_rope_bwd(*(t.detach() for t in (dout, qkv)), None, None, pos, f, 2, EPS)
     assert not dqkv.requires_grad and dw.shape == (0, 16)
+
+
+@pytest.mark.parametrize("which", ["qkv", "k_pages", "v_pages", "q_w", "inv_freq", "q", "ak_pages", "av_pages"])
+def test_forward_mode_tangents_are_refused(which):
+    """A tangent on any input of the paged operators, which have no derivative, raises instead of being dropped, without
+    gradients enabled too; a tangent that forward mode itself ignores does not."""
+    import torch.autograd.forward_ad as fw
+
+    o = ops()
+    m, i = dict(device="meta"), dict(device="meta", dtype=torch.int32)
+    t = dict(qkv=torch.empty(2, 3, 96, **m), k_pages=torch.empty(4, 2, 16, 16, **m), v_pages=torch.empty(4, 2, 16, 16, **m),
+             q_w=torch.empty(16, **m), inv_freq=torch.empty(8, **m), q=torch.empty(2, 3, 32, **m))
+    t.update(ak_pages=t["k_pages"], av_pages=t["v_pages"])
+    table, past, e = torch.empty(2, 2, **i), torch.empty(2, **i), torch.empty(2, device="meta", dtype=torch.int64)
+
+    def call(t):
+        if which in ("q", "ak_pages", "av_pages"):
+            return o.attn_decode_shared(t["q"], t["ak_pages"], t["av_pages"], None, None, table, past, None, 0, 16, 0, e)
+        return o.kv_append_paged(t["qkv"], t["k_pages"], t["v_pages"], table, past, None, t["q_w"], torch.empty(16, **m),
+                                 torch.empty(2, 3, **m), t["inv_freq"], EPS, e)
+
+    assert call(t).shape == (2, 3, 32)
+    with fw.dual_level():
+        dual = {**t, which: fw.make_dual(t[which], torch.empty_like(t[which]))}
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="no gradient"):
+                call(dual)
+        with fw._set_fwd_grad_enabled(False):
+            assert call(dual).shape == (2, 3, 32)
+        with pytest.raises(RuntimeError, match="jvp"):
+            o.qk_norm_rope_bwd(t["qkv"], t["qkv"], fw.make_dual(t["q_w"], torch.empty_like(t["q_w"])), t["q_w"], None, None, 2,
+                               EPS)
