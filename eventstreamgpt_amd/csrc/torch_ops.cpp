@@ -803,17 +803,40 @@ void no_gradient(const char* what, const Ts&... ts) {
                               "forward-mode tangent)");
 }
 
+Tensor call_append(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                   const Tensor& past, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
+                   const optional<Tensor>& k_w, const optional<Tensor>& pos, const optional<Tensor>& inv_freq, double eps,
+                   const Tensor& err) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("esgpt::kv_append_paged", "")
+                       .typed<decltype(kv_append_paged)>();
+  return op.call(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err);
+}
+
 Tensor kv_append_paged_autograd(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
                                 const Tensor& past, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
                                 const optional<Tensor>& k_w, const optional<Tensor>& pos,
                                 const optional<Tensor>& inv_freq, double eps, const Tensor& err) {
   auto t = [](const optional<Tensor>& x) { return x.has_value() ? *x : Tensor(); };
   no_gradient("kv_append_paged", qkv, k_pages, v_pages, t(q_w), t(k_w), t(pos), t(inv_freq));
-  static auto op = c10::Dispatcher::singleton()
-                       .findSchemaOrThrow("esgpt::kv_append_paged", "")
-                       .typed<decltype(kv_append_paged)>();
-  at::AutoDispatchBelowADInplaceOrView guard;
-  return op.call(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err);
+  at::AutoDispatchBelowAutograd guard;
+  return call_append(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err);
+}
+
+// The pools' versions count the write, as any in-place operator's: a graph that saved a pool before it does not run
+// backward on what the append stored. (Inference tensors have no version.)
+Tensor kv_append_paged_in_place(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                                const Tensor& past, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
+                                const optional<Tensor>& k_w, const optional<Tensor>& pos,
+                                const optional<Tensor>& inv_freq, double eps, const Tensor& err) {
+  Tensor q;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    q = call_append(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err);
+  }
+  for (const Tensor* p : {&k_pages, &v_pages})
+    if (!p->is_inference()) torch::autograd::impl::bump_version(*p);
+  return q;
 }
 
 Tensor attn_decode_shared_autograd(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
@@ -1510,6 +1533,10 @@ TORCH_LIBRARY_IMPL(esgpt, CUDA, m) {
   m.impl("pack", &pack);
   m.impl("adamw", &adamw);
   m.impl("adamw_dev", &adamw_dev);
+}
+
+TORCH_LIBRARY_IMPL(esgpt, ADInplaceOrView, m) {
+  m.impl("kv_append_paged", &kv_append_paged_in_place);
 }
 
 TORCH_LIBRARY_IMPL(esgpt, Autograd, m) {

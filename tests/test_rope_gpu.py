@@ -588,3 +588,29 @@ def test_forward_mode_tangents_are_refused(which):
         with pytest.raises(RuntimeError, match="jvp"):
             o.qk_norm_rope_bwd(t["qkv"], t["qkv"], fw.make_dual(t["q_w"], torch.empty_like(t["q_w"])), t["q_w"], None, None, 2,
                                EPS)
+
+
+def test_an_append_counts_as_a_write_to_the_pools():
+    """Both pools' versions grow with each append, in inference mode too, so that a graph which saved a pool refuses to run
+    backward after it; inference tensors, which have no version, are taken as ever."""
+    o = ops()
+    i = dict(device="meta", dtype=torch.int32)
+    kp, vp = (torch.empty(4, 2, 16, 16, device="meta") for _ in range(2))
+
+    def append(kp, vp):
+        return o.kv_append_paged(torch.empty(2, 3, 96, device="meta"), kp, vp, torch.empty(2, 2, **i), torch.empty(2, **i),
+                                 None, None, None, None, None, EPS, torch.empty(2, device="meta", dtype=torch.int64))
+
+    w = torch.empty(4, 2, 16, 16, device="meta", requires_grad=True)
+    for n, mode in enumerate((torch.enable_grad, torch.no_grad, torch.inference_mode)):
+        loss = [(w * pool).sum() for pool in (kp, vp)]
+        with mode():
+            assert append(kp, vp).shape == (2, 3, 32)
+        assert kp._version == vp._version == n + 1
+        for at in loss:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                at.backward()
+    with torch.inference_mode():
+        ki, vi = kp.clone(), vp.clone()
+        append(ki, vi)
+    append(ki, vi)
