@@ -681,7 +681,7 @@ void refuse_capture_with(const Tensor& leaf) {
 Tensor qk_norm_rope_autograd(const Tensor& qkv, const optional<Tensor>& q_w, const optional<Tensor>& k_w,
                              const optional<Tensor>& pos, const optional<Tensor>& inv_freq, int64_t H, double eps) {
   for (const auto* t : {&pos, &inv_freq})
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->has_value() || !(*t)->defined() || !(*t)->requires_grad(),
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->has_value() || !tracked(**t),
                                 "eventstreamgpt_amd: qk_norm_rope has no gradient for pos and inv_freq");
   if (at::GradMode::is_enabled()) {
     refuse_capture_with(qkv);

@@ -614,3 +614,15 @@ def test_an_append_counts_as_a_write_to_the_pools():
         ki, vi = kp.clone(), vp.clone()
         append(ki, vi)
     append(ki, vi)
+
+
+def test_frequencies_that_are_parameters():
+    """pos and inv_freq that require a gradient are refused where one is recorded, and only there."""
+    o = ops()
+    qkv, q_w, k_w, pos, f = inputs(2, 3, 2, 16, 16, torch.float32, dev="meta")
+    for kw in (dict(inv_freq=torch.nn.Parameter(f), pos=pos), dict(inv_freq=f, pos=pos.clone().requires_grad_())):
+        with pytest.raises(NotImplementedError, match="no gradient for pos and inv_freq"):
+            o.qk_norm_rope(qkv, q_w, k_w, H=2, eps=EPS, **kw)
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode():
+                assert not o.qk_norm_rope(qkv, q_w, k_w, H=2, eps=EPS, **kw).requires_grad
