@@ -670,6 +670,8 @@ __global__ __launch_bounds__(64 * kWaves, KD * NT < 8 ? 2 : 1) void shared_kerne
     const int id = (int)(blockIdx.x - a.units) * kWaves + w;
     const int ch = id % a.NSc, sh = id / a.NSc, h = sh % a.H, s = sh / a.H;
     if (s >= a.S) return;
+    // a bound of 0 leaves no history workgroup to see a length beyond it
+    if (a.units == 0 && a.prefix_lens && a.prefix_lens[s / a.n] != 0) set_err(a.err, ESGPT_FLAG_BAD_PAGE);
     const W x(a, h, lds + w * kTile);
     OneSegment<1> sg;
     sg.tab = a.table + (int64_t)s * a.table_w;

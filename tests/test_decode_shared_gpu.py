@@ -691,3 +691,21 @@ def test_scores_of_any_size(c, dt):
                 r = int(x.past[s]) // 2
                 want = x.vp[x.table[s, r // x.ps], :, r % x.ps].expand(x.Lq, -1, -1)
                 assert torch.equal(got[s], want), (scale, top, s)
+
+
+@gpu
+def test_a_history_beyond_a_bound_of_zero_is_flagged():
+    """prefix_cap = 0 (PagedKV.attend's default) with a history: nothing of it is seen, and that is said; histories of no
+    rows are within the bound."""
+    from eventstreamgpt_amd import kernels as K
+
+    x = Case(2, 3, 1, 2, 32, 16, 64, 32)
+    got = x.run(prefix_cap=0)
+    with pytest.raises(IndexError, match="paged cache"):
+        K.check_errors()
+    empty = x.run(prefix_cap=0, prefix_lens=torch.zeros(2).int())
+    assert torch.equal(got, empty)
+    x.P = 0
+    x.check(got)
+    assert torch.equal(got, x.run())
+    K.check_errors()
