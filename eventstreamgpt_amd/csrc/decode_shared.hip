@@ -56,6 +56,7 @@ struct SharedArgs {
   int S, n, Lq, H, hd, psl;     // psl: log2 of the page size
   int prefix_cap, cap;
   int window, owin;             // the window where it can cut the history, the own rows (0: never)
+  uint32_t far;                 // the window of a row beyond the cap
   int M, RT, tr;                // rows of a group; row tiles of the history's workgroups; whole form: rows of a tile
   int NPc, NSc, NP, pchunk, schunk;
   int units;  // history workgroups; the own rows' follow
@@ -95,11 +96,12 @@ __device__ __forceinline__ int cols_max(int v) { return -cols_min(-v); }
 
 // One new event: its place among its trajectory's own rows. active: it exists, is not padding and its past is sane.
 struct Row {
-  int at;  // own row
+  uint32_t at;  // own row
+  bool far;     // it lies beyond the cap: a window still counts from it
   bool active;
 };
 __device__ __forceinline__ Row row_of(const SharedArgs& a, int s, int i, bool exists) {
-  Row r{0, false};
+  Row r{0, false, false};
   if (!exists) return r;
   const int past = a.past[s];
   int k = i;
@@ -110,14 +112,21 @@ __device__ __forceinline__ Row row_of(const SharedArgs& a, int s, int i, bool ex
     keep = a.row_mask[(int64_t)s * a.Lq + i] != 0;
   }
   if (!keep) return r;
-  if (past < 0 || past > a.cap - 1 - k) {  // a row that the cache has no place for
+  r.far = past > a.cap - 1 - k;
+  if (past < 0 || r.far) {  // a row that the cache has no place for
     set_err(a.err, ESGPT_FLAG_BAD_PAGE);
     if (past < 0) return r;
   }
-  r.at = min(past, a.cap) + k;
+  r.at = (uint32_t)past + k;
   r.active = true;
   return r;
 }
+// How many of the first `end` rows lie before the window of the row that has n - 1 rows before it, and how many up to it.
+__device__ __forceinline__ int rows_before(const SharedArgs& a, const Row& r, uint32_t n, int window, int end) {
+  const uint32_t w = r.far ? a.far : window ? (uint32_t)window : ~0u;
+  return (int)min((uint32_t)end, n - min(n, w));
+}
+__device__ __forceinline__ int rows_to(uint32_t n, int end) { return (int)min((uint32_t)end, n); }
 __device__ __forceinline__ int prefix_len(const SharedArgs& a, int g) {
   if (a.prefix_cap == 0) return 0;
   const int P = a.prefix_lens[g];
@@ -681,9 +690,10 @@ __global__ __launch_bounds__(64 * kWaves, KD * NT < 8 ? 2 : 1) void shared_kerne
     x.load_q(q[0], (int64_t)s * a.Lq + c, c < a.Lq);
     const Row r = row_of(a, s, c, c < a.Lq);
     sg.act[0] = r.active;
-    sg.hi[0] = r.active ? min(r.at + 1, a.cap) : 0;
-    sg.lo[0] = (r.active && a.owin) ? max(0, r.at - a.owin + 1) : 0;
-    const int base = cols_min(r.active ? sg.lo[0] : a.cap) & ~15, end = cols_max(sg.hi[0]);  // no active row: no key
+    sg.hi[0] = r.active ? rows_to(r.at + 1, a.cap) : 0;
+    sg.lo[0] = r.active ? rows_before(a, r, r.at + 1, a.owin, a.cap) : 0;
+    const int base = a.owin ? cols_min(r.active ? sg.lo[0] : a.cap) & ~15 : 0;
+    const int end = cols_max(sg.hi[0]);  // no active row: no key
     sg.first = base + ch * a.schunk;
     sg.end = min(end, sg.first + a.schunk);
     if (a.owin && sg.first < sg.end) sg.raw = x.pages(sg.tab, sg.first, W::KB, sg.end);
@@ -725,7 +735,7 @@ __global__ __launch_bounds__(64 * kWaves, KD * NT < 8 ? 2 : 1) void shared_kerne
     const Row r = row_of(a, grp * a.n + rr / a.Lq, rr % a.Lq, rr < a.M);
     sg.act[t] = r.active;
     sg.hi[t] = r.active ? P : 0;
-    sg.lo[t] = (r.active && a.window) ? min(P, max(0, P + r.at - a.window + 1)) : 0;
+    sg.lo[t] = r.active ? rows_before(a, r, P + r.at + 1, a.window, P) : 0;
     if (r.active) base = min(base, sg.lo[t]);
   }
   // chunks count from the first row that a window of this group can reach, whatever its own rows
@@ -762,6 +772,7 @@ __global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
     const SharedArgs& a;
     const int32_t* ptab;
     int w, s0, count, P, my, plo, phi, olo, ohi, ids;
+    int pfrom, ofrom;  // where a walk begins: no later than where the page ids that it was given do
     bool act;
     __device__ __forceinline__ int seq(int seg) const { return s0 + (NW - 1 - w) + (seg - 1) * NW; }
     __device__ __forceinline__ int stride(int seg) const { return seg == 0 ? NW * W::KB : W::KB; }
@@ -771,11 +782,11 @@ __global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
     __device__ __forceinline__ void open(const W& x, int seg, int& k0, int& k_end, int& raw) {
       raw = ids;
       if (seg == 0) {
-        k0 = w * W::KB + (cols_min(act ? plo : P) & ~15);
+        k0 = w * W::KB + (cols_min(act ? pfrom : P + 15) & ~15);  // no active row: no key
         k_end = P;
       } else {
         const bool mine = act && my == seq(seg);
-        k0 = cols_min(mine ? olo : a.cap) & ~15;
+        k0 = cols_min(mine ? ofrom : a.cap) & ~15;
         k_end = cols_max(mine ? ohi : 0);
       }
       if (seg == 0 ? a.window : a.owin) {
@@ -810,9 +821,11 @@ __global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
   const Row r = row_of(a, sg.my, rr % a.Lq, exists);
   sg.act = r.active;
   sg.phi = r.active ? sg.P : 0;
-  sg.plo = (r.active && a.window) ? min(sg.P, max(0, sg.P + r.at - a.window + 1)) : 0;
-  sg.ohi = r.active ? min(r.at + 1, a.cap) : 0;
-  sg.olo = (r.active && a.owin) ? max(0, r.at - a.owin + 1) : 0;
+  sg.plo = r.active ? rows_before(a, r, sg.P + r.at + 1, a.window, sg.P) : 0;
+  sg.ohi = r.active ? rows_to(r.at + 1, a.cap) : 0;
+  sg.olo = r.active ? rows_before(a, r, r.at + 1, a.owin, a.cap) : 0;
+  sg.pfrom = a.window ? sg.plo : 0;
+  sg.ofrom = a.owin ? sg.olo : 0;
   State<1, W::DT> st;
   x.walk(st, q, sg);
   J::run(a, st, 0, r.active, lds, out0, rt * a.tr, a.tr, h, 0);
@@ -1029,6 +1042,7 @@ int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_p
   auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
   ESGPT_REQUIRE(q && o && past && page_table && aligned(q) && aligned(o) && (prefix_cap == 0 || (prefix_table && prefix_lens)));
   ESGPT_REQUIRE(n_pages == 0 || (k_pages && v_pages && aligned(k_pages) && aligned(v_pages)));
+  const uint32_t far = window ? (uint32_t)std::min<int64_t>(window, ~0u) : ~0u;
   window = cut_window(window, prefix_cap, cap);
   const SharedPlan p = shared_plan(G, S, Lq, H, hd, prefix_cap, cap, window, dtype);
   // a launch holds fewer than 2^32 threads
@@ -1066,6 +1080,7 @@ int esgpt_attn_decode_shared(const void* q, const void* k_pages, const void* v_p
   a.cap = (int)cap;
   a.window = (int)window;
   a.owin = window < cap ? (int)window : 0;
+  a.far = far;
   a.M = (int)((S / G) * Lq);
   a.RT = p.RT;
   a.tr = p.tr;

@@ -709,3 +709,31 @@ def test_a_history_beyond_a_bound_of_zero_is_flagged():
     x.check(got)
     assert torch.equal(got, x.run())
     K.check_errors()
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", [(2, 3, 2, 2, 32, 16, 64, 32, 20), (2, 3, 1, 2, 64, 16, 64, 37, 50), (16, 3, 1, 8, 96, 16, 90, 12, 20),
+                               (1, 6, 3, 2, 64, 64, 9001, 700, 300), (3, 2, 1, 2, 16, 16, 0, 70, 33), (32, 3, 2, 4, 128, 16, 70, 20, 100),
+                               (2, 3, 1, 2, 24, 16, 64, 37, 200)], ids=str)
+def test_windows_of_a_past_beyond_its_bound(c, dt):
+    """A length beyond its bound is flagged, and what lies there counts as not visible: a window still counts from the row
+    itself and not from the bound. Pasts that leave some of the bounded rows in the window, and none."""
+    from eventstreamgpt_amd import kernels as K
+
+    x = Case(*c, dt=dt)
+    clean = x.run()
+    K.check_errors()
+    far = [x.s, x.s + x.window // 2, x.s + x.window, x.s + x.window + x.P, 2**30, 2**31 - 1]
+    for i, past in enumerate(far):
+        x.past[i % x.S] = past
+        want = x.oracle()
+        got = x.run()
+        x.check(got, want)
+        with pytest.raises(IndexError, match="paged cache"):
+            K.check_errors()
+        if past >= x.s + x.window + x.P:
+            assert (got[i % x.S] == 0).all()
+        keep = torch.ones(x.S, dtype=torch.bool)  # the other groups; a group's walk begins where its rows' windows do
+        keep[: (min(i, x.S - 1) // x.n + 1) * x.n] = False
+        assert torch.equal(got[keep.to(DEV)], clean[keep.to(DEV)])
