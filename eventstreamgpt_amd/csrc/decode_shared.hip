@@ -756,8 +756,11 @@ __global__ __launch_bounds__(64 * kWaves, KD * NT < 8 ? 2 : 1) void shared_kerne
 // the result. The waves take every NW-th block of the history (segment 0) and, from the other end, every NW-th
 // trajectory's own rows, which only that trajectory's columns see; a segment's page ids are loaded when the one before is
 // opened.
+//
+// Four waves (above 64 dimensions): two workgroups a CU, at most 256 registers. Left to itself f32 at 128 dimensions took 292,
+// and one workgroup a CU: 16 x 64 over 1,000 + 20, 8 heads, 110 us against 79.
 template <typename T, int KD, int NW>
-__global__ __launch_bounds__(64 * NW) void shared_whole_kernel(SharedArgs a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void shared_whole_kernel(SharedArgs a) {
   using W = Walk<T, KD>;
   using J = Join<T, KD, NW>;
   constexpr int kTile = W::kBf16 ? W::KB * W::LD * 2 : 0;
@@ -900,9 +903,10 @@ int block_keys(int64_t hd, int dtype) {
 //     (f32 1.6) a step and workgroup of a CU, 32 rows a tile 1.6 (2.6), + 0.002 a block of own rows; all by a block's
 //     bytes / 16 KB.
 //     One full round, or short histories: 32x8 512+24 window 32 h8 8.3 / 14.3; 32x16 1000+20 h8 20.7 / 24.0, f32 39.6 /
-//       42.6; 32x16 512+128 h8 f32 55.0 / 64.7; 32x128 256+64 h4 62.6 / 70.0; 32x64 256+20 h4 hd128 27.6 / 56.6
+//       42.6; 32x16 512+128 h8 f32 55.0 / 64.7; 32x128 256+64 h4 62.6 / 70.0; 32x64 256+20 h4 hd128 26.5 / 40.8, f32 46.5 /
+//       67.5; f32 hd128 16x64 1000+20 h8 79 / 99, 64x16 256+64 h8 104 / 118
 //     A round begun for a few workgroups: 33x8 1500+20 h8 35.5 / 29.0; 20x32 2000+20 h8 41.4 / 31.0; 24x40 2000+20 h8
-//       f32 hd128 240 / 174. Many row tiles over a long history: 8x64 two events 4096+20 h8 52.5 / 35.0, 32x40 two
+//       f32 hd128 190 / 171. Many row tiles over a long history: 8x64 two events 4096+20 h8 52.5 / 35.0, 32x40 two
 //       3000+20 h8 114 / 85.0
 //     One wave's chain of own rows: 64x1 512+400 h8 34.9 / 24.9, 64x2 39.3 / 34.8
 // Without a history the split form's waves are the whole of it, and write directly where one chunk holds a trajectory.

@@ -60,3 +60,11 @@ def test_no_scratch_spills_in_product_kernels():
         hits = [k for k in ks if re.search(pat, k["name"])]
         assert hits, pat
         assert all(k.get("private_segment_fixed_size", 0) == 0 for k in hits), pat
+
+
+def test_whole_form_of_the_shared_decode_attention_fits_its_plan():
+    """Its plan counts on two waves a SIMD: one workgroup of eight waves a CU, or two of four. That is 256 registers (of both
+    kinds) a lane at most."""
+    ks = [k for k in _kernels() if "shared_whole_kernel" in k["name"]]
+    assert len(ks) == 8
+    assert [(k["name"], k["vgpr_count"]) for k in ks if k["vgpr_count"] > 256] == []
