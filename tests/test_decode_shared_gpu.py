@@ -737,3 +737,97 @@ def test_windows_of_a_past_beyond_its_bound(c, dt):
         keep = torch.ones(x.S, dtype=torch.bool)  # the other groups; a group's walk begins where its rows' windows do
         keep[: (min(i, x.S - 1) // x.n + 1) * x.n] = False
         assert torch.equal(got[keep.to(DEV)], clean[keep.to(DEV)])
+
+
+# ------------------------------------------------------------------- forms that the rule takes and no test above reaches
+WHOLE = [  # G, n, Lq, H, hd, ps, P, s, window: one launch without a workspace, in both types
+    (8, 32, 1, 16, 32, 64, 11560, 1685, 0),   # more blocks a wave, in the history and in an own segment, than page ids come at once
+    (8, 32, 1, 16, 32, 64, 16000, 1685, 15000), (8, 32, 1, 16, 24, 16, 300, 1700, 0), (8, 32, 1, 16, 32, 64, 900, 1690, 1300),
+    (32, 32, 2, 4, 128, 64, 256, 64, 0), (16, 64, 1, 8, 128, 64, 1000, 20, 0), (32, 64, 1, 4, 100, 64, 256, 20, 100),
+]
+
+
+def test_the_whole_form_is_what_those_cases_take():
+    """No workspace with a history: the whole form. In f32 at 128 dimensions, and with more than 32 (f32), 16 (bf16) blocks
+    a wave and segment, which is what one load of page ids reaches."""
+    import os
+
+    from eventstreamgpt_amd import _lib as L
+
+    if not os.path.exists(L.LIB_PATH):
+        pytest.skip("library not built")
+    need = L.load(require_device=False).esgpt_attn_decode_shared_workspace
+    for G, n, Lq, H, hd, ps, P, s, window in WHOLE:
+        for dt in (L.F32, L.BF16):
+            hd = -(-hd // 8) * 8 if dt == L.BF16 else hd
+            assert need(G, G * n, Lq, H, hd, P, s, window, dt) == 0, (G, n, hd, P, s, dt)
+    # keys of a block: 32 in f32, 64 in bf16; eight waves share a history, one takes an own segment; 64 page ids a load, one a
+    # 16-key tile
+    for kb, per in ((32, 32), (64, 16)):
+        assert -(-11560 // (8 * kb)) > per and -(-1685 // kb) > per
+
+
+def whole_case(c, dt, **kw):
+    return Case(*(c if c[4] % 8 == 0 or dt == F32 else (*c[:4], -(-c[4] // 8) * 8, *c[5:])), dt=dt, share=True, **kw)
+
+
+def check_some(x, got, c, dt, masked, want_of=lambda y: y.oracle(), seqs=None):
+    """The oracle's answer for a few sequences of a case whose tables all name the same pages."""
+    for s in seqs or sorted({0, 1, x.n, x.S // 2 + 3, x.S - 1}):
+        y = whole_case(c, dt, masked=masked)
+        y.kp, y.vp = x.kp, x.vp
+        y.S = y.G = y.n = 1
+        y.prefix_table, y.prefix_lens = x.prefix_table[s // x.n: s // x.n + 1], x.prefix_lens[s // x.n: s // x.n + 1]
+        y.table, y.past, y.q = x.table[s: s + 1], x.past[s: s + 1], x.q[s: s + 1]
+        y.row_mask = None if x.row_mask is None else x.row_mask[s: s + 1]
+        y.check(got[s: s + 1], want_of(y))
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", WHOLE, ids=str)
+def test_whole_form_over_long_segments_and_wide_heads(c, dt):
+    masked = c[2] > 1
+    x = whole_case(c, dt, masked=masked)
+    got = x.run()
+    check_some(x, got, c, dt, masked)
+    if masked:
+        assert (got[~x.row_mask.to(DEV)] == 0).all()
+    assert int(err()[0]) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", [WHOLE[4], WHOLE[6]], ids=str)
+def test_whole_form_keeps_what_is_not_finite_to_the_rows_that_see_it(c, dt):
+    """128 and 100 dimensions, padded rows: NaN beyond every length, an infinity at an own row that only some sequences are
+    long enough to see."""
+    masked = c[2] > 1
+    x = whole_case(c, dt, masked=masked)
+    P, t = int(x.prefix_lens.max()), x.s // 2
+    clean = x.run()
+    for pool in (x.kp, x.vp):
+        # every table names the same pages: what no sequence reaches
+        for tab, last in ((x.prefix_table[0], P), (x.table[0], int(x.past.max()) + x.Lq)):
+            for i, page in enumerate(tab.tolist()):
+                pool[page, :, min(max(last - i * x.ps, 0), x.ps):] = math.nan
+    assert torch.equal(x.run(), clean)
+    x.vp[x.table[0, t // x.ps], 1, t % x.ps, 9] = math.inf
+    got = x.run().view(x.S, x.Lq, x.H, -1)
+    at = torch.tensor([[x.own_row(s, i) for i in range(x.Lq)] for s in range(x.S)])
+    active = torch.ones(x.S, x.Lq, dtype=torch.bool) if x.row_mask is None else x.row_mask
+    sees = active & (at >= t) & ((at - t < x.window) if x.window else torch.ones_like(active))
+    assert sees.any() and not sees.all()
+    assert (got[..., 1, 9].cpu()[sees] == math.inf).all() and torch.isfinite(got[..., 1, 9].cpu()[~sees]).all()
+    got[..., 1, 9] = torch.where(sees.to(DEV), clean.view(got.shape)[..., 1, 9], got[..., 1, 9])
+
+    def want(y):
+        vp = y.vp
+        y.vp = vp.clone()
+        y.vp[x.table[0, t // x.ps], 1, t % x.ps, 9] = clean_value
+        out = y.oracle()
+        y.vp = vp
+        return out
+
+    clean_value = float(whole_case(c, dt, masked=masked).vp[x.table[0, t // x.ps], 1, t % x.ps, 9])
+    check_some(x, got.view(x.S, x.Lq, -1), c, dt, masked, want, [0, int((~sees).any(1).nonzero()[0]), x.S - 1])
