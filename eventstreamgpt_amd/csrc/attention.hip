@@ -659,13 +659,26 @@ __global__ __launch_bounds__(256) void attn_bwd_small4(
     if (bh >= W) break;  // wave-uniform
     const S4Item<T, VE, LKM>& cur = it[t];
     const int64_t h = bh % H, b = bh / H;
-    float dka[LKM][VE], dva[LKM][VE];
+    constexpr int KEPT = ONE ? 1 : LKM;
+    float dka[KEPT][VE], dva[KEPT][VE];
 #pragma unroll
-    for (int j = 0; j < LKM; ++j)
+    for (int j = 0; j < KEPT; ++j)
 #pragma unroll
       for (int e = 0; e < VE; ++e) dka[j][e] = dva[j][e] = 0.f;
+    // dK / dV of key j: the four query groups' partials summed (every group ends with the sums); group j % 4 stores them
+    auto finish = [&](int j, float(&ka)[VE], float(&va)[VE]) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        ka[e] = cross_rows(ka[e]);
+        va[e] = cross_rows(va[e]);
+      }
+      if ((j & 3) == g) {
+        store_vec<T, VE>(dk + (b * Lk + j) * ld_d + h * hd + c, ka);
+        store_vec<T, VE>(dv + (b * Lk + j) * ld_d + h * hd + c, va);
+      }
+    };
     // ONE (Lq <= 4): a single query block, no loop — the packed operands are widened where they are used instead
-    // of being hoisted out of a loop as f32 copies
+    // of being hoisted out of a loop as f32 copies, and a key's dK / dV are stored as soon as they are known
     for (int64_t i0 = 0; i0 < (ONE ? 1 : Lq); i0 += 4) {
       const int64_t i = i0 + g;
       const bool qin = i < Lq;
@@ -706,17 +719,25 @@ __global__ __launch_bounds__(256) void attn_bwd_small4(
         }
         sv = row_sum16(sv);
         dpv = row_sum16(dpv);
-        if (!(qvalid && ((cur.km >> j) & 1u) && j >= jlo && j <= pos)) continue;  // row-uniform
-        const float keep = dr.p > 0.f ? small_keep<I32>(dr, bh, Lq, Lk, ii, j) : 1.f;
-        const float p = expf(sv - ls);
-        const float ds = p * (dpv * keep - dl);
-        const float pd = p * keep;
+        if constexpr (ONE) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          dqa[e] = fmaf(ds, raw_at<T, VE>(cur.k[j], e), dqa[e]);
-          dka[j][e] = fmaf(ds, qr[e], dka[j][e]);
-          dva[j][e] = fmaf(pd, dor[e], dva[j][e]);
+          for (int e = 0; e < VE; ++e) dka[0][e] = dva[0][e] = 0.f;
         }
+        if (qvalid && ((cur.km >> j) & 1u) && j >= jlo && j <= pos) {  // row-uniform
+          const float keep = dr.p > 0.f ? small_keep<I32>(dr, bh, Lq, Lk, ii, j) : 1.f;
+          const float p = expf(sv - ls);
+          const float ds = p * (dpv * keep - dl);
+          const float pd = p * keep;
+          float(&ka)[VE] = dka[ONE ? 0 : j];
+          float(&va)[VE] = dva[ONE ? 0 : j];
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            dqa[e] = fmaf(ds, raw_at<T, VE>(cur.k[j], e), dqa[e]);
+            ka[e] = fmaf(ds, qr[e], ka[e]);
+            va[e] = fmaf(pd, dor[e], va[e]);
+          }
+        }
+        if constexpr (ONE) finish(j, dka[0], dva[0]);
       }
       if (qin) store_vec<T, VE>(dq + (b * tq + ii) * ld_d + h * hd + c, dqa);
     }
@@ -727,19 +748,11 @@ __global__ __launch_bounds__(256) void attn_bwd_small4(
       for (int e = 0; e < VE; ++e) z[e] = 0.f;
       store_vec<T, VE>(dq + (b * tq - 1 - g) * ld_d + h * hd + c, z);
     }
-    // dK / dV: the four query groups' partials summed (every group ends with the sums); group g stores the rows
-    // j = g, g + 4
+    if constexpr (!ONE) {
 #pragma unroll
-    for (int j = 0; j < LKM; ++j) {
-      if (j >= Lk) break;  // wave-uniform
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        dka[j][e] = cross_rows(dka[j][e]);
-        dva[j][e] = cross_rows(dva[j][e]);
-      }
-      if ((j & 3) == g) {
-        store_vec<T, VE>(dk + (b * Lk + j) * ld_d + h * hd + c, dka[j]);
-        store_vec<T, VE>(dv + (b * Lk + j) * ld_d + h * hd + c, dva[j]);
+      for (int j = 0; j < LKM; ++j) {
+        if (j >= Lk) break;  // wave-uniform
+        finish(j, dka[j], dva[j]);
       }
     }
   }

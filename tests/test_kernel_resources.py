@@ -68,3 +68,15 @@ def test_whole_form_of_the_shared_decode_attention_fits_its_plan():
     ks = [k for k in _kernels() if "shared_whole_kernel" in k["name"]]
     assert len(ks) == 8
     assert [(k["name"], k["vgpr_count"]) for k in ks if k["vgpr_count"] > 256] == []
+
+
+def test_dependency_graph_attention_backward_keeps_its_waves():
+    """One query block per item, head size 64: the waves a SIMD that bound it, five up to six tokens (102 registers) and
+    four up to eight (128), in both types."""
+    seen = 0
+    for k in _kernels():
+        m = re.search(r"attn_bwd_small4I(?:f|14__hip_bfloat16)Li4ELi([468])ELb[01]ELi1ELb1E", k["name"])
+        if m:
+            seen += 1
+            assert k["vgpr_count"] <= (128 if m.group(1) == "8" else 102), (k["name"], k["vgpr_count"])
+    assert seen == 8
