@@ -540,12 +540,20 @@ RopeIn rope_in(const char* what, const Tensor& x, int64_t rows0, int64_t rows1, 
 const void* vptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 const float* fptr(const Tensor& t) { return t.defined() ? ptr<const float>(t) : nullptr; }
 
+void check_hd(const char* what, at::ScalarType t, int64_t H, int64_t hd, int64_t most = INT64_MAX) {
+  const int64_t step = t == at::kBFloat16 ? 8 : 4;
+  TORCH_CHECK(hd > 0 && hd <= 128 && hd % step == 0 && H <= most / hd, what, ": invalid argument: ", H, " heads of ", hd,
+              ": a head size is a multiple of ", step, " in this type and at most 128",
+              most < INT64_MAX ? ", H * head size at most " + std::to_string(most) : std::string());
+}
+
 // Head size of a packed [B, T, 3D] buffer, checked.
 int64_t packed_hd(const char* what, const Tensor& qkv, int64_t H) {
   require_hip(qkv, "qkv");
   dtype_code(qkv.scalar_type());
   TORCH_CHECK(qkv.dim() == 3 && H > 0 && qkv.size(2) % (3 * H) == 0 && qkv.size(2) > 0, what,
               ": qkv must be [B, T, 3 * H * head size] with H = ", H);
+  check_hd(what, qkv.scalar_type(), H, qkv.size(2) / 3 / H, 16384);
   return qkv.size(2) / 3 / H;
 }
 
@@ -783,6 +791,7 @@ Tensor attn_decode_shared(const Tensor& q_, const Tensor& k_pages, const Tensor&
   Tensor q = rows16(q_);
   Tensor o = at::empty({S, Lq, H * hd}, q.options());
   if (o.numel() == 0) return o;
+  check_hd(what, q.scalar_type(), H, hd);
   const int dt = dtype_code(q.scalar_type());
   const size_t nb = esgpt_attn_decode_shared_workspace(G, S, Lq, H, hd, prefix_cap, cap, window, dt);
   const c10::DataPtr ws = scratch(nb);

@@ -626,3 +626,24 @@ def test_frequencies_that_are_parameters():
         for mode in (torch.no_grad, torch.inference_mode):
             with mode():
                 assert not o.qk_norm_rope(qkv, q_w, k_w, H=2, eps=EPS, **kw).requires_grad
+
+
+@gpu
+def test_unsupported_head_sizes_are_named():
+    """The refusal says which head size is not supported and what the rule is, at every entry point."""
+    i = dict(device=DEV, dtype=torch.int32)
+    for dt, H, hd, step in ((torch.float32, 2, 136, 4), (torch.bfloat16, 2, 12, 8), (torch.float32, 1, 6, 4),
+                            (torch.bfloat16, 129, 128, 8)):
+        qkv, rule = torch.zeros(1, 1, 3 * H * hd, device=DEV, dtype=dt), f"{H} heads of {hd}: a head size is a multiple of {step} "
+        kp, vp = (torch.zeros(1, H, 16, hd, device=DEV, dtype=dt) for _ in range(2))
+        table, past = torch.zeros(1, 1, **i), torch.zeros(1, **i)
+        calls = [lambda: ops().qk_norm_rope(qkv, None, None, None, None, H, EPS),
+                 lambda: ops().qk_norm_rope_bwd(qkv, qkv, None, None, None, None, H, EPS),
+                 lambda: ops().kv_append_paged(qkv, kp, vp, table, past, None, None, None, None, None, EPS, err())]
+        for call in calls:
+            with pytest.raises(RuntimeError, match=rule):
+                call()
+        if H < 129:
+            with pytest.raises(RuntimeError, match=f"heads of {hd}: a head size is a multiple of {step} "):
+                ops().attn_decode_shared(torch.zeros(1, 1, H * hd, device=DEV, dtype=dt), kp, vp, None, None, table, past, None, 0,
+                                         16, 0, err())
