@@ -682,8 +682,8 @@ void refuse_capture_with(const Tensor& leaf) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(reinterpret_cast<hipStream_t>(stream_of(leaf)), &st) != hipSuccess) (void)hipGetLastError();
   TORCH_CHECK(st == hipStreamCaptureStatusNone, "eventstreamgpt_amd: qk_norm_rope is captured while an eager graph of the "
-              "same leaves, made on the default stream, is alive: its backward could not be captured (delete that graph, or "
-              "make it on the capturing stream)");
+              "same leaves, made on the default stream, is alive: its backward could not be captured (delete that graph, "
+              "make it on the capturing stream, or capture under torch.no_grad() if no backward is to be captured)");
 }
 
 Tensor qk_norm_rope_autograd(const Tensor& qkv, const optional<Tensor>& q_w, const optional<Tensor>& k_w,

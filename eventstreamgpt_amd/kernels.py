@@ -667,7 +667,9 @@ class PagedKV:
     (``esgpt::kv_append_paged``) and ``attend`` attends them (``esgpt::attn_decode_shared``). A generation with ``n``
     trajectories per subject stores each subject's history once, under ``prefix_table``::
 
-        q = cache.append(history_qkv, prefix_table, zero, row_mask=event_mask, ...)     # [B, L, 3D], once
+        y = qk_norm_rope(history_qkv, ...)                                               # [B, L, 3D], once
+        o = attention(y, event_mask, ...)                                                # the prompt's own attention
+        cache.append(y, prefix_table, zero, row_mask=event_mask)                         # as it is
         for each new event:                                                              # [B * n, 1, 3D]
             q = cache.append(qkv, page_table, past, ...)
             o = cache.attend(q, page_table, past, cap, prefix_table, event_mask.sum(1).int(), L)

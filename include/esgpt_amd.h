@@ -235,7 +235,8 @@ int esgpt_attn_decode(const void* q, int64_t ld_q, const void* k_cache, const vo
  *   f64: the product is exact, event times reach 1e6 minutes); v is copied. out is what esgpt_attn_fwd reads, whose
  *   scores are not scaled by 1/sqrt(hd). pos: [N], pos_dtype ESGPT_POS_F32 / _I64; inv_freq: f32 [R/2]; R = 0: no
  *   rotation (pos, inv_freq may be NULL). hd <= 128, hd % 8 == 0 (bf16) or hd % 4 == 0 (f32), H*hd <= 16384, R even
- *   and <= hd; 16-B aligned buffers; out apart from qkv.
+ *   and <= hd; 16-B aligned buffers; out apart from qkv. Accesses are as wide (16 B at most) as R/2 and (hd - R)/2 are
+ *   multiples of: an odd R/2 makes them one element.
  * esgpt_qk_norm_rope_bwd: from the raw rows and dout [N, 3D]: dqkv [N, 3D] and, with weights,
  *   dw f32 [2, hd] = (d q_w, d k_w), summed in a fixed order (workspace: esgpt_qk_norm_rope_bwd_workspace bytes).
  * esgpt_kv_append_paged: the same norm and rotation of S sequences' new rows qkv [S, Lq, 3D] on the way into a paged

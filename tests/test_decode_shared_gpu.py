@@ -831,3 +831,31 @@ def test_whole_form_keeps_what_is_not_finite_to_the_rows_that_see_it(c, dt):
 
     clean_value = float(whole_case(c, dt, masked=masked).vp[x.table[0, t // x.ps], 1, t % x.ps, 9])
     check_some(x, got.view(x.S, x.Lq, -1), c, dt, masked, want, [0, int((~sees).any(1).nonzero()[0]), x.S - 1])
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+def test_a_normalised_prompt_is_stored_as_it_is(dt):
+    """A prompt that was normalised and rotated for its own attention is stored without weights and positions: the pools
+    get the bits that an append with them leaves, and the queries are the prompt's own."""
+    from eventstreamgpt_amd import kernels as K
+
+    B, L, H, hd, ps = 3, 45, 4, 64, 16
+    D = H * hd
+    g = torch.Generator().manual_seed(7)
+    rows = torch.randn(B, L, 3 * D, generator=g).to(dt).to(DEV)
+    times = torch.exp(3 + torch.randn(B, L, generator=g)).cumsum(1).to(DEV)
+    mask = (torch.arange(L)[None] >= torch.tensor([0, 17, 44])[:, None]).to(DEV)
+    w = [(hd**-0.25 * (1 + 0.2 * torch.randn(hd, generator=g))).to(DEV) for _ in range(2)]
+    f = torch.exp(torch.arange(0, hd, 2) * (-math.log(10000.0) / hd)).float().to(DEV)
+    a, b = (K.PagedKV(9, ps, H, hd, dt, DEV) for _ in range(2))
+    table, zero = a.pages(9).view(3, 3), torch.zeros(B, dtype=torch.int32, device=DEV)
+    for pool in (a.k, a.v, b.k, b.v):
+        pool.zero_()
+    y = K.qk_norm_rope(rows, *w, times, f, H)
+    q = a.append(rows, table, zero, mask, *w, times, f)
+    q2 = b.append(y, table, zero, mask)
+    assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v) and torch.equal(q, q2)
+    assert torch.equal(q, torch.where(mask[..., None], y[..., :D], torch.zeros_like(q)))
+    assert K.attention(y, mask, None, H, 0, False).shape == (B, L, D)
+    K.check_errors()
