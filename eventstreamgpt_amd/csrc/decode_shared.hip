@@ -10,8 +10,8 @@
 // MFMAs, where lane l holds column (query row) l % 16 and keys 4 (l / 16) .. + 3 of a 16-key tile, so a row's softmax
 // statistics are lane-local but for two lane swaps, and P goes from the accumulator to the next product's operand
 // without leaving its lane. An own row is one column of sixteen: 15/16 of the MFMA rate idles there, which costs
-// nothing as long as memory is the bound (a bf16 tile of 16 keys x 64 takes 64 MFMA cycles for 4 KB, 64 B per cycle and
-// SIMD, against the 13 B per cycle that HBM gives a whole CU).
+// nothing as long as memory is the bound (a bf16 tile of 16 keys x 64 takes 96 MFMA cycles, two thirds of them for the two
+// parts of P (Walk::pv), for 4 KB: 43 B per cycle and SIMD, against the 13 B per cycle that HBM gives a whole CU).
 //
 // Two forms (shared_plan chooses and holds the measurements). Whole: one workgroup per (group, head, 4..16 rows) does the
 // history and the own rows and writes the result. Split: the history of each (group, head, 16 or 32 rows) is cut into
@@ -23,7 +23,7 @@
 // descriptors. Measured with those in vector registers (a wave's number taken from threadIdx, a length loaded like data),
 // every buffer load became a loop over the lanes: 3,555 vector instructions a wave against 1,622, 32 x 16 over 256 + 64
 // events 15.5 us against 13.1; 64 keys a block rather than 32, 8 x 32 over 16,384 events 59.5 -> 58.9 at 512 chunks.
-// Now 8 x 32 over 16,384 + 64 (hd 64, 8 heads, bf16) takes 52 us + 4 of join: 5.0 TB/s, what a large copy reaches.
+// Now 8 x 32 over 16,384 + 64 (hd 64, 8 heads, bf16) takes MAIN us + JOIN of join.
 //
 // Nothing is read beyond a sequence's length: rows past it are zeros in registers, so what an unused part of a page
 // holds (NaN, infinity) never meets a product. Where a tile is partly masked (a window's edge, a later event of the same
@@ -887,38 +887,39 @@ int block_keys(int64_t hd, int dtype) {
 // workgroup and one workgroup of eight waves (above 64 dimensions two of four) a CU at a time; its rounds cost what its
 // busiest wave's chain of blocks costs (steps: those of the history and those of its trajectories' own rows). A tile is
 // 16 rows, or 8 or 4 while there are fewer workgroups than CUs: the history is then read by more of them, out of L2,
-// and each has fewer trajectories (32x16 256+64: 16 rows 12.9, 8 rows 11.4). Measured in graph replays, whole / split
+// and each has fewer trajectories (32x16 256+64 h4: 16 rows 13.8, 8 rows 11.8). Measured in graph replays, whole / split
 // us (groups x trajectories, history + own rows, heads; hd 64 bf16 if not said):
 //   the busiest wave's chain of blocks is short: one; two in bf16 if half the waves have no history; up to 32 dimensions
-//     one more, three in bf16. In a graph 8x4 100+10 h4 6.8 / 7.9; 1x4 40+6 h4 f32 hd16 6.3 / 7.2; 4x4 100+100 h4 8.4 /
-//     9.1; 8x30 3+5 h1 hd128 8.4 / 8.7; 4x16 500+60 h4 hd32 7.8 / 7.9; 4x8 200+20 h4 f32 hd16 8.1 / 7.7; 5x2 691+109 h8
-//     hd16 8.2 / 7.6; 3x5 900+50 h4 hd16 8.6 / 7.6. A call that is not in a graph pays 3 us of host time for the second
-//     launch and its workspace: the last four 7.8 / 10.4, 8.1 / 10.6, 8.3 / 10.7, 8.7 / 10.6. Longer chains lose: 8x8
-//     400+40 h4 9.4 / 8.6, 1x8 600+30 h8 9.8 / 8.4, 16x4 87+288 h2 hd24 10.0 / 7.6, 8x4 300+30 h4 hd128 11.9 / 9.8, f32
-//     4x16 256+64 h4 13.2 / 11.2, 2x13 106+189 h5 hd16 12.2 / 7.9
-//   smaller tiles for half the CUs or more, and a chain of at most three: 32x16 256+64 h4 11.4 / 15.0; 32x8 256+64 h4
-//     9.1 / 11.5; 16x16 256+64 h4 f32 14.1 / 14.9 (a longer history: 4x16 1000+20 h8 12.3 / 9.9, 4x64 2048+32 h8 18.8 /
-//     16.7)
+//     one more, three in bf16. In a graph 8x4 100+10 h4 7.1 / 8.4; 1x4 40+6 h4 f32 hd16 6.4 / 7.2; 4x4 100+100 h4 9.0 /
+//     9.5; 8x30 3+5 h1 hd128 8.7 / 8.9. At the rule's end a replayed call loses, 4x16 500+60 h4 hd32 8.2 / 8.0; 4x8 200+20
+//     h4 f32 hd16 8.1 / 7.7; 2x13 106+189 h5 hd16 8.7 / 7.9; 5x2 691+109 h8 hd16 8.8 / 7.7; 3x5 900+50 h4 hd16 9.1 / 7.8,
+//     and an eager one, which pays 3 us of host time for the second launch and its workspace, gains more: 8.5 / 11.4, 8.2 /
+//     11.4, 9.1 / 11.8, 9.1 / 11.6, 9.5 / 11.5. Longer chains lose: 8x8 400+40 h4 10.0 / 9.0, 1x8 600+30 h8 10.4 / 8.8,
+//     16x4 87+288 h2 hd24 10.8 / 7.8, 8x4 300+30 h4 hd128 12.3 / 9.9, f32 4x16 256+64 h4 13.3 / 11.3, f32 2x13 106+189 h5
+//     hd16 12.2 / 8.0
+//   smaller tiles for half the CUs or more, and a chain of at most three: 32x16 256+64 h4 11.8 / 15.2; 32x8 256+64 h4
+//     9.3 / 11.7; 16x16 256+64 h4 f32 14.1 / 15.3 (a longer history: 4x16 1000+20 h8 13.3 / 10.4, 4x64 2048+32 h8 18.8 /
+//     17.4)
 //   16-row tiles for every CU: by an estimate of both in us. Whole: 8 + 2.8 (f32 3.2) a step and round. Split: 14 + 1.2
 //     (f32 1.6) a step and workgroup of a CU, 32 rows a tile 1.6 (2.6), + 0.002 a block of own rows; all by a block's
 //     bytes / 16 KB.
-//     One full round, or short histories: 32x8 512+24 window 32 h8 8.3 / 14.3; 32x16 1000+20 h8 20.7 / 24.0, f32 39.6 /
-//       42.6; 32x16 512+128 h8 f32 55.0 / 64.7; 32x128 256+64 h4 62.6 / 70.0; 32x64 256+20 h4 hd128 26.5 / 40.8, f32 46.5 /
-//       67.5; f32 hd128 16x64 1000+20 h8 79 / 99, 64x16 256+64 h8 104 / 118
-//     A round begun for a few workgroups: 33x8 1500+20 h8 35.5 / 29.0; 20x32 2000+20 h8 41.4 / 31.0; 24x40 2000+20 h8
-//       f32 hd128 190 / 171. Many row tiles over a long history: 8x64 two events 4096+20 h8 52.5 / 35.0, 32x40 two
-//       3000+20 h8 114 / 85.0
-//     One wave's chain of own rows: 64x1 512+400 h8 34.9 / 24.9, 64x2 39.3 / 34.8
+//     One full round, or short histories: 32x8 512+24 window 32 h8 9.0 / 15.2; 32x16 1000+20 h8 21.3 / 25.3, f32 36.9 /
+//       38.6; 32x16 512+128 h8 f32 55.1 / 62.6; 32x128 256+64 h4 63.8 / 76.8; 32x64 256+20 h4 hd128 27.2 / 41.1, f32 46.5 /
+//       67.5; f32 hd128 16x64 1000+20 h8 79.9 / 99.3, 64x16 256+64 h8 103 / 119
+//     A round begun for a few workgroups: 33x8 1500+20 h8 37.5 / 29.7; 20x32 2000+20 h8 44.3 / 31.8; 24x40 2000+20 h8
+//       f32 hd128 191 / 172. Many row tiles over a long history: 8x64 two events 4096+20 h8 54.6 / 39.4, 32x40 two
+//       3000+20 h8 119 / 89.6
+//     One wave's chain of own rows: 64x1 512+400 h8 38.6 / 27.1, 64x2 41.7 / 35.8
 // Without a history the split form's waves are the whole of it, and write directly where one chunk holds a trajectory.
-// The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 55.8 / 58.8, 8x8 8192+32 h8 f32
-// 50.7 / 52.2, 16x4 1024+33 h4 f32 15.0 / 18.2, 4x64 2048+32 h8 16.9 / 20.1 (more parts cost more joins); own rows at
+// The split form's chunks aim at one workgroup per CU: 256 / 512 units 8x32 16384+64 h8 57.4 / 59.4, 8x8 8192+32 h8 f32
+// 51.3 / 53.9, 16x4 1024+33 h4 f32 16.5 / 17.2, 24x40 2000+20 h8 47.5 / 53.1 (more parts cost more joins); own rows at
 // 1,024 waves: 16x16 256+64 f32 15.7 against 19.7 at 4,096. In f32 up to 32 dimensions a workgroup has little in
-// flight, and two a CU pay: 8x32 8192+32 h8 hd32 55.1 -> 42.2, 2x64 4096+32 h8 hd16 16.9 -> 15.0 (bf16 19.3 -> 20.6,
+// flight, and two a CU pay: 8x32 8192+32 h8 hd32 45.5 -> 38.4, 2x64 4096+32 h8 hd16 17.0 -> 14.9 (bf16 19.3 -> 20.6,
 // 10.7 -> 10.6).
 // History tiles of 32 rows halve the reads but leave half the workgroups to share a history; they pay where each wave
-// still has 256 keys. 16 / 32 rows: 24x40 2000+20 h8 51.3 / 46.0, 20x32 2000 32.2 / 30.9, 4x32 16384 h8 f32 78.6 /
-// 66.1, 16x32 4096 f32 83.4 / 71.4; fewer: 4x20 1000 h4 9.1 / 10.8, 1x40 6000 h8 13.3 / 14.4, 8x32 2048 f32 27.8 /
-// 28.4. At 128 dimensions (f32: above 64) two accumulators leave one wave a SIMD: 24x40 2000 h8 77.3 / 96.4, 1x40 6000
+// still has 256 keys. 16 / 32 rows: 24x40 2000+20 h8 53.1 / 47.2, 20x32 2000 33.9 / 31.9, 4x32 16384 h8 f32 79.4 /
+// 65.2, 16x32 4096 f32 83.9 / 71.2; fewer: 4x20 1000 h4 9.5 / 11.1, 1x40 6000 h8 14.0 / 15.1, 8x32 2048 f32 29.0 /
+// 27.7. At 128 dimensions (f32: above 64) two accumulators leave one wave a SIMD: 24x40 2000 h8 77.3 / 96.4, 1x40 6000
 // 18.5 / 25.7.
 SharedPlan shared_plan(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap, int64_t cap,
                        int64_t window, int dtype) {

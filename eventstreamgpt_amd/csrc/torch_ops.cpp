@@ -822,16 +822,6 @@ Tensor call_append(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pag
   return op.call(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err);
 }
 
-Tensor kv_append_paged_autograd(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
-                                const Tensor& past, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
-                                const optional<Tensor>& k_w, const optional<Tensor>& pos,
-                                const optional<Tensor>& inv_freq, double eps, const Tensor& err) {
-  auto t = [](const optional<Tensor>& x) { return x.has_value() ? *x : Tensor(); };
-  no_gradient("kv_append_paged", qkv, k_pages, v_pages, t(q_w), t(k_w), t(pos), t(inv_freq));
-  at::AutoDispatchBelowAutograd guard;
-  return call_append(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err);
-}
-
 // The pools' versions count the write, as any in-place operator's: a graph that saved a pool before it does not run
 // backward on what the append stored. (Inference tensors have no version.)
 Tensor kv_append_paged_in_place(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
@@ -846,6 +836,17 @@ Tensor kv_append_paged_in_place(const Tensor& qkv, const Tensor& k_pages, const 
   for (const Tensor* p : {&k_pages, &v_pages})
     if (!p->is_inference()) torch::autograd::impl::bump_version(*p);
   return q;
+}
+
+// The next kernel is the one above: called here, a dispatch less.
+Tensor kv_append_paged_autograd(const Tensor& qkv, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                                const Tensor& past, const optional<Tensor>& row_mask, const optional<Tensor>& q_w,
+                                const optional<Tensor>& k_w, const optional<Tensor>& pos,
+                                const optional<Tensor>& inv_freq, double eps, const Tensor& err) {
+  no_gradient("kv_append_paged", qkv, k_pages, v_pages);
+  for (const auto* t : {&q_w, &k_w, &pos, &inv_freq})
+    if (t->has_value()) no_gradient("kv_append_paged", **t);
+  return kv_append_paged_in_place(qkv, k_pages, v_pages, page_table, past, row_mask, q_w, k_w, pos, inv_freq, eps, err);
 }
 
 Tensor attn_decode_shared_autograd(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
