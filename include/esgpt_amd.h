@@ -267,9 +267,10 @@ int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, c
  * q [S, Lq, D] and the new events' own rows as esgpt_kv_append_paged left them (the same past and row_mask); o
  * [S, Lq, D]: zeros in padded rows. prefix_table int32 [G, prefix_w] / page_table int32 [S, table_w] name pages of one
  * pool. prefix_cap / cap: bounds on the prefix lengths and on past + new that the work is split by (at most the tables'
- * room; prefix_cap = 0: no history, prefix_table / prefix_lens may be NULL); a length beyond its bound, a negative one
- * or a page outside the pool raises ESGPT_FLAG_BAD_PAGE, and what lies there counts as not visible. Rows beyond a length
- * are never read. A row whose visible scores are all -inf gives zeros. workspace: esgpt_attn_decode_shared_workspace
+ * room; prefix_cap = 0: no history, prefix_table / prefix_lens may be NULL, and a prefix_lens[g] > 0 is beyond the bound);
+ * a length beyond its bound, a negative one or a page outside the pool raises ESGPT_FLAG_BAD_PAGE, and what lies there
+ * counts as not visible (a new event beyond cap sees the rows within cap that its window, counted from its own place,
+ * leaves). Rows beyond a length are never read. A row whose visible scores are all -inf gives zeros. workspace: esgpt_attn_decode_shared_workspace
  * bytes (0: none needed). */
 size_t esgpt_attn_decode_shared_workspace(int64_t G, int64_t S, int64_t Lq, int64_t H, int64_t hd, int64_t prefix_cap,
                                           int64_t cap, int64_t window, int dtype);
