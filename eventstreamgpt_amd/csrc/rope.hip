@@ -569,6 +569,10 @@ int esgpt_kv_append_paged(const void* qkv, const float* q_w, const float* k_w, c
   if (S * Lq == 0) return ESGPT_OK;
   ESGPT_REQUIRE(past && q && aligned16(q) && (table_w == 0 || page_table) &&
                 (n_pages == 0 || (k_pages && v_pages && aligned16(k_pages) && aligned16(v_pages))));
+  // one pool for both, or pools that overlap: keys and values would overwrite each other in no order
+  const uintptr_t pool = (uintptr_t)n_pages * H * page_size * hd * (dtype == ESGPT_BF16 ? 2 : 4), kp = (uintptr_t)k_pages,
+                  vp = (uintptr_t)v_pages;
+  ESGPT_REQUIRE((kp < vp ? vp - kp : kp - vp) >= pool);
   const Plan p = make_plan(S * Lq, H, hd, R, dtype, MODE_APPEND);
   RopeArgs a = rope_args(p, qkv, q_w, k_w, pos, pos_dtype, inv_freq, R, S * Lq, H, hd, eps, dtype);
   a.out = q;

@@ -742,6 +742,8 @@ Tensor kv_append_paged(const Tensor& qkv_, const Tensor& k_pages, const Tensor& 
   const char* what = "esgpt.kv_append_paged";
   check_pages(what, qkv_, k_pages, v_pages);
   const int64_t H = k_pages.size(1), hd = packed_hd(what, qkv_, H), S = qkv_.size(0), Lq = qkv_.size(1);
+  const auto kp = reinterpret_cast<uintptr_t>(k_pages.data_ptr()), vp = reinterpret_cast<uintptr_t>(v_pages.data_ptr());
+  TORCH_CHECK((kp < vp ? vp - kp : kp - vp) >= k_pages.nbytes(), what, ": k_pages and v_pages overlap");
   TORCH_CHECK(hd == k_pages.size(3), what, ": the pages hold heads of ", k_pages.size(3), ", qkv of ", hd);
   const c10::DeviceGuard guard(qkv_.device());
   const RopeIn r = rope_in(what, qkv_, S, Lq, hd, q_w, k_w, pos, inv_freq);

@@ -241,7 +241,7 @@ int esgpt_attn_decode(const void* q, int64_t ld_q, const void* k_cache, const vo
  *   dw f32 [2, hd] = (d q_w, d k_w), summed in a fixed order (workspace: esgpt_qk_norm_rope_bwd_workspace bytes).
  * esgpt_kv_append_paged: the same norm and rotation of S sequences' new rows qkv [S, Lq, 3D] on the way into a paged
  *   cache. k_pages / v_pages: [n_pages, H, page_size, hd] (a head's rows of one page are contiguous; page_size a
- *   power of two, 16..65536); page_table int32 [S, table_w]. Row i of sequence s goes to cache row past[s] + (rows
+ *   power of two, 16..65536; the two pools apart); page_table int32 [S, table_w]. Row i of sequence s goes to cache row past[s] + (rows
  *   before i that row_mask [S, Lq] keeps; NULL: all), i.e. padded rows are not stored; q [S, Lq, D] gets the
  *   normalised, rotated queries (zeros in padded rows). Lq <= 2^24, S * Lq <= 2^31 - 1024. A row beyond the table, a
  *   negative past or a page outside [0, n_pages) raises ESGPT_FLAG_BAD_PAGE and is not stored. Cache rows must be

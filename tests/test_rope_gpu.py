@@ -647,3 +647,30 @@ def test_unsupported_head_sizes_are_named():
             with pytest.raises(RuntimeError, match=f"heads of {hd}: a head size is a multiple of {step} "):
                 ops().attn_decode_shared(torch.zeros(1, 1, H * hd, device=DEV, dtype=dt), kp, vp, None, None, table, past, None, 0,
                                          16, 0, err())
+
+
+@gpu
+def test_overlapping_pools_are_refused():
+    """One tensor for both pools, or two views that share rows: keys and values would overwrite each other in no order.
+    Neighbouring halves of one tensor are two pools."""
+    S, Lq, H, hd, ps = 2, 3, 2, 16, 16
+    qkv, q_w, k_w, pos, f = inputs(S, Lq, H, hd, 16, torch.float32)
+    both = torch.zeros(8, H, ps, hd, device=DEV)
+    table, past = torch.arange(4, device=DEV).view(2, 2).int(), torch.zeros(2, device=DEV).int()
+    for kp, vp in ((both[:4], both[:4]), (both[:4], both[3:7]), (both[3:7], both[:4])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops().kv_append_paged(qkv, kp, vp, table, past, None, q_w, k_w, pos, f, EPS, err())
+    assert (both == 0).all()
+    kp, vp = cache(4, H, ps, hd, torch.float32)
+    both[4:], both[:4] = kp, vp
+    want = ops().kv_append_paged(qkv, kp, vp, table, past, None, q_w, k_w, pos, f, EPS, err())
+    got = ops().kv_append_paged(qkv, both[4:], both[:4], table, past, None, q_w, k_w, pos, f, EPS, err())
+    assert torch.equal(got, want) and torch.equal(both[4:], kp) and torch.equal(both[:4], vp)
+
+
+def test_c_abi_refuses_overlapping_pools():
+    lib = _lib()
+    P = 1 << 20  # never read
+    size = 4 * 4 * 64 * 64 * 2
+    for vp in (P, P + size - 16, P - size + 16):
+        assert lib.esgpt_kv_append_paged(P, P, P, P, 0, P, 64, 1e-6, None, P, P, 2, P, vp, 4, 64, P, 2, 1, 4, 64, 1, None, None) == 1
