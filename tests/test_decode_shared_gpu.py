@@ -859,3 +859,12 @@ def test_a_normalised_prompt_is_stored_as_it_is(dt):
     assert torch.equal(q, torch.where(mask[..., None], y[..., :D], torch.zeros_like(q)))
     assert K.attention(y, mask, None, H, 0, False).shape == (B, L, D)
     K.check_errors()
+
+
+@gpu
+@pytest.mark.parametrize("c", [(2, 5, 1, 3, 4, 16, 70, 21, 0), (2, 3, 2, 2, 12, 16, 130, 20, 30), (16, 9, 1, 8, 20, 32, 100, 40, 0),
+                               (1, 6, 1, 2, 68, 64, 3000, 300, 0), (32, 3, 2, 4, 124, 16, 70, 20, 0)], ids=str)
+def test_f32_heads_that_are_multiples_of_four(c):
+    x = Case(*c, dt=F32)
+    x.check(x.run())
+    assert int(err()[0]) == 0

@@ -674,3 +674,48 @@ def test_c_abi_refuses_overlapping_pools():
     size = 4 * 4 * 64 * 64 * 2
     for vp in (P, P + size - 16, P - size + 16):
         assert lib.esgpt_kv_append_paged(P, P, P, P, 0, P, 64, 1e-6, None, P, P, 2, P, vp, 4, 64, P, 2, 1, 4, 64, 1, None, None) == 1
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(3, 5, 1, 4, 4), (2, 33, 7, 12, 8), (1, 9, 3, 20, 2), (2, 6, 2, 124, 100), (5, 3, 1, 100, 0)],
+                         ids=str)
+def test_f32_heads_that_are_multiples_of_four(shape):
+    """Through a normalising append and back: the operator on rows, its backward, the append and the pools' rows."""
+    B, T, H, hd, R = shape
+    qkv, q_w, k_w, pos, f = inputs(B, T, H, hd, R, torch.float32)
+    y = ops().qk_norm_rope(qkv, q_w, k_w, pos, f, H, EPS)
+    x, w = qkv.double().requires_grad_(), [t.double().requires_grad_() for t in (q_w, k_w)]
+    want = oracle(x, *w, pos, f, H)
+    close(y, want.detach(), torch.float32, want.abs().max().item() * math.sqrt(2))
+    dout = torch.randn(qkv.shape, generator=torch.Generator().manual_seed(1)).to(DEV)
+    grads = torch.autograd.grad(want, [x, *w], dout.double())
+    dqkv, dw = ops().qk_norm_rope_bwd(dout, qkv, q_w, k_w, pos, f, H, EPS)
+    xs = qkv[..., : 2 * H * hd].double().view(B, T, 2 * H, hd)
+    r = torch.rsqrt(xs.pow(2).mean(-1) + EPS).max().item() * max(t.abs().max().item() for t in (q_w, k_w))
+    close(dqkv, grads[0], torch.float32, 2 * r * dout.double().abs().max().item() * math.sqrt(2), 96)
+    xh = (xs.view(B, T, 2, H, hd) * torch.rsqrt(xs.view(B, T, 2, H, hd).pow(2).mean(-1, keepdim=True) + EPS)).abs()
+    mag = (xh * math.sqrt(2) * dout.double().abs().max()).sum((0, 1, 3))
+    for i in range(2):
+        assert ((dw[i].double() - grads[1 + i]).abs() <= (24 + 64 + B * T * H) * U * mag[i]).all()
+    kp, vp = cache(B * 4, H, 16, hd, torch.float32)
+    table, past = torch.randperm(B * 4, generator=torch.Generator().manual_seed(2)).view(B, 4).int(), torch.arange(B).int() * 5
+    wq, wk, wv = append_oracle(y, kp, vp, table, past, None, H)
+    q = ops().kv_append_paged(qkv, kp, vp, table.to(DEV), past.to(DEV), None, q_w, k_w, pos, f, EPS, err())
+    assert torch.equal(q, wq) and torch.equal(kp, wk) and torch.equal(vp, wv) and int(err()[0]) == 0
+
+
+@gpu
+def test_one_weight_for_queries_and_keys():
+    """A weight that both share gets the sum of both gradients; in two calls of one graph, of all four."""
+    B, T, H, hd, R = 2, 9, 3, 32, 32
+    qkv, q_w, _, pos, f = inputs(B, T, H, hd, R, torch.float32)
+    dout = torch.randn_like(qkv)
+    _, dw = ops().qk_norm_rope_bwd(dout, qkv, q_w, q_w, pos, f, H, EPS)
+    q_w.requires_grad_()
+    (ops().qk_norm_rope(qkv, q_w, q_w, pos, f, H, EPS) * dout).sum().backward()
+    assert torch.equal(q_w.grad, dw[0] + dw[1])
+    once, q_w.grad = q_w.grad.clone(), None
+    a = ops().qk_norm_rope(qkv, q_w, q_w, pos, f, H, EPS)
+    b = ops().qk_norm_rope(qkv, q_w, q_w, pos, f, H, EPS)
+    ((a + b) * dout).sum().backward()
+    assert (q_w.grad - 2 * once).abs().max() <= 4 * U * 2 * (dw[0].abs() + dw[1].abs()).max()
